@@ -121,6 +121,7 @@ int souffle_workspace_status(void *workspace, souffle_stream_t stream, unsigned 
  * which cpp/bert/test_souffle_bert_layer.py:131-143,161 loads; the reference's own kernels compute the tanh form
  * (cpp/bert/bert_base_impl.cu:722-734) or ReLU (cpp/bert/kernels/fused_sqq_feedforward.cu:327-341). */
 enum { SOUFFLE_ACT_GELU_TANH = 0, SOUFFLE_ACT_RELU = 1, SOUFFLE_ACT_GELU_ERF = 2 };
+enum { SOUFFLE_ACT_NONE = 3 };   /* of the 8-bit linear layers only */
 
 typedef struct {
   int batch, seq_len;          /* runtime; seq_len <= 512.  Lengths other than 64/128/256/384/512 run as the next of
@@ -383,6 +384,79 @@ int souffle_pointwise_conv2d_bn(const void *x, const void *w, const float *scale
 int souffle_depthwise_conv2d_bn_swish(const void *x, const void *w, const float *scale, const float *shift,
                                       void *y, int in_h, int in_w, int channels, int kernel, int stride,
                                       souffle_stream_t stream);
+
+/* ------------------------------------- rows of fp16, bf16 and fp32 activations ---- */
+/* The operators below have no counterpart in the reference.  They take activations of three types, compute in fp32 and
+ * round once; rows lie `ld` ELEMENTS apart (ld >= their length) and may start at any multiple of the element's size.
+ * A call with no rows does nothing.  None of them keeps anything between calls, and none waits for another workgroup:
+ * they may overlap with anything, and be captured into graphs. */
+enum { SOUFFLE_F16 = 0, SOUFFLE_BF16 = 1, SOUFFLE_F32 = 2 };
+
+/* ------------------------------------------------- 8-bit linear layers ---- */
+/* y = act(s[m] t[n] sum_k q[m][k] w[k][n] + bias[n]): rows in 8-bit integers with one scale per row, weights with one per
+ * output channel; the sums are exact 32-bit integers.  K <= 131071.
+ * A row x becomes q = round_half_even(x / s) with s = max(fp32(max |x| / 127), 2^-100): the rounding of the real quotient.
+ * A row that holds a NaN or an infinity gets s = NaN (and q = 0), so that all results computed from it are NaN.
+ * q lies in rows of ldq bytes, ldq a multiple of 16 and at least K rounded up to 64; the bytes behind K are multiplied
+ * by zeros, whatever they hold.
+ * Weights are kept packed (souffle_int8_packed_bytes = K and N rounded up to 64, multiplied; 16-byte aligned), made once
+ * when a model is loaded: the bytes of weight (k, n) lie at
+ *     ((n / 64 * ceil(K / 64) + k / 64) * 4 + n / 4 % 4) * 1024 + (k / 16 % 4 * 16 + n / 16 % 4 * 4 + n % 4) * 16 + k % 16
+ * and the rest is zero.  bias (nullable) and y are of type `dtype`.  act: SOUFFLE_ACT_*. */
+size_t souffle_int8_packed_bytes(int K, int N);
+/* packs w [K][N] (rows ldw apart) of 8-bit integers that a caller brings with their scales */
+int souffle_int8_pack_weight(const int8_t *w, long long ldw, void *packed, int K, int N, souffle_stream_t stream);
+/* quantises w [K][N] of `dtype` per column by the rule for rows above, and packs it */
+int souffle_int8_quantize_weight(const void *w, int dtype, long long ldw, void *packed, float *col_scale, int K, int N, souffle_stream_t stream);
+int souffle_quantize_rows(const void *x, int dtype, long long ldx, int8_t *q, long long ldq, float *row_scale, int M, int K,
+                          souffle_stream_t stream);
+int souffle_gemm_int8(const int8_t *q, long long ldq, const float *row_scale, const void *packed, const float *col_scale,
+                      const void *bias, int act, void *y, int dtype, long long ldy, int M, int N, int K, souffle_stream_t stream);
+/* Both steps in one call, x [M][K] of `dtype`; same result, bit for bit.  The workspace holds the quantised rows during
+ * the call and needs no initialisation. */
+size_t souffle_linear_int8_workspace_bytes(int M, int K);
+int souffle_linear_int8(const void *x, long long ldx, const void *packed, const float *col_scale, const void *bias, int act, void *y,
+                        int dtype, long long ldy, int M, int N, int K, void *workspace, size_t workspace_bytes, souffle_stream_t stream);
+
+/* --------------------------------------------------------- gated norm ---- */
+/* Between two blocks of a transformer, per row of `cols` elements:
+ *     y = residual_scale * x + gate * N_post(f)        x: the residual stream, f: the block's output
+ *     h = N_pre(y)                                     the next block's input, from y before y is rounded
+ * N is (v - mean) / sqrt(var + eps) (LAYER) or v / sqrt(mean v^2 + eps) (RMS), times gamma, plus beta; N_post may be
+ * absent (NONE).  With post_norm NONE, no gate and residual_scale 1, h is a post-norm encoder's LN(x + f). */
+enum { SOUFFLE_NORM_NONE = 0, SOUFFLE_NORM_LAYER = 1, SOUFFLE_NORM_RMS = 2 };
+typedef struct {
+  int rows, cols;                /* cols <= 16384 */
+  int dtype;                     /* SOUFFLE_F16 / BF16 / F32: of the rows and of all vectors */
+  int post_norm, pre_norm;       /* SOUFFLE_NORM_*; pre_norm is LAYER or RMS */
+  int rows_per_gate;             /* consecutive rows that share one row of gate (a sequence); 0: all rows share one */
+  float residual_scale, post_eps, pre_eps;
+  long long ldx, ldf, ldy, ldh;  /* in elements */
+} souffle_gated_norm_cfg;
+typedef struct {                 /* [cols] each, gate [rows / rows_per_gate][cols]; any may be NULL (gamma, gate 1; beta 0) */
+  const void *post_gamma, *post_beta, *gate, *pre_gamma, *pre_beta;
+} souffle_gated_norm_w;
+/* y may be NULL (not wanted); y may be x or f, and h may be f or x, in place (same pointer and stride). */
+int souffle_gated_norm_forward(const souffle_gated_norm_cfg *cfg, const souffle_gated_norm_w *w, const void *x, const void *f,
+                               void *y, void *h, souffle_stream_t stream);
+/* The same with h handed over as 8-bit rows (see souffle_quantize_rows; h is not rounded before): q [rows][ldq], ldq a
+ * multiple of 16 and at least cols rounded up to 64 (bytes behind cols are left undefined), row_scale [rows]. */
+int souffle_gated_norm_forward_int8(const souffle_gated_norm_cfg *cfg, const souffle_gated_norm_w *w, const void *x, const void *f,
+                                    void *y, int8_t *q, long long ldq, float *row_scale, souffle_stream_t stream);
+/* Gradients for incoming dy and dh (either may be NULL: zero).  Every output may be NULL (not wanted); the vectors'
+ * gradients have the vectors' shapes and type, are summed in fp32 in a fixed order (two calls give the same bits) and
+ * are rounded once.  dx may be dy and df may be dh in place.  rows must not be 0.  The workspace
+ * (souffle_gated_norm_backward_workspace_bytes, needed where a vector's gradient is wanted) holds partial sums during
+ * the call; it needs no initialisation. */
+typedef struct {
+  void *dx, *df;
+  void *pre_gamma, *pre_beta, *gate, *post_gamma, *post_beta;
+  long long ld_dy, ld_dh, ld_dx, ld_df;      /* in elements */
+} souffle_gated_norm_grad;
+size_t souffle_gated_norm_backward_workspace_bytes(const souffle_gated_norm_cfg *cfg);
+int souffle_gated_norm_backward(const souffle_gated_norm_cfg *cfg, const souffle_gated_norm_w *w, const void *dy, const void *dh,
+                                const void *x, const void *f, const souffle_gated_norm_grad *grad, void *workspace,
+                                size_t workspace_bytes, souffle_stream_t stream);
 
 /* ------------------------------------------------------------- timing ---- */
 /* Replaces benchmarkCudaFunc (cpp/souffle_utils/cuda_utils.h:102-136): after `warmup`

@@ -1,0 +1,607 @@
+// The norms on both sides of a block, its gate and the residual scale as one pass over the rows, and their gradients.
+//
+//   forward    p = N_post(f), y = a x + g * p, h = N_pre(y)       per row of D elements, statistics in fp32
+//   backward   dh -> dyt = dy + N_pre'(dh), dx = a dyt, dg = sum dyt p, df = N_post'(dyt g), and the vectors' gradients
+//
+// Both are bound by memory: 2 + 2 row arrays of traffic forward, 4 + 2 backward, against some 20 and 50 operations an
+// element.  A row lives in the registers of TPR threads (8 NV elements each) between its one load and its one store; the
+// vectors (gamma, beta, gate) stay in registers over the rows a workgroup walks, as they would otherwise be read from
+// the L2 once per row, as often as the rows themselves.  h is computed from y before y is rounded.
+#include <algorithm>
+#include "typed.hpp"
+#include "host_util.hpp"
+
+namespace souffle {
+namespace gated_norm {
+
+struct FwdArgs {
+  const void *x, *f, *post_gamma, *post_beta, *gate, *pre_gamma, *pre_beta;
+  void *y, *h;                      // y nullable
+  int8_t *q;                        // instead of h: the row in 8-bit integers
+  float *q_scale;
+  long long ldx, ldf, ldy, ldh, ldq;
+  int rows, cols, post, pre, rows_per_gate, rows_per_slot;
+  float a, post_eps, pre_eps;
+};
+
+// Sum over the TPR threads of a row.  `red` has two halves that are used in turn, so one barrier per sum is enough: a
+// wave that writes half i again has passed the barrier of the sum in between, behind which nobody reads half i any more.
+template <int TPR>
+struct RowReduce {
+  static constexpr int kWaves = TPR / 64;
+  unsigned *red;                    // [2][kWaves] of this row slot
+  int turn;
+  __device__ __forceinline__ float sum(float v) {
+    v = wave_sum_dpp(v);
+    if constexpr (kWaves == 1) return v;
+    float *r = reinterpret_cast<float *>(red) + turn * kWaves;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) r[(threadIdx.x / 64) % kWaves] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s += r[w];
+    return s;
+  }
+  __device__ __forceinline__ unsigned umax(unsigned v) {
+    v = wave_umax_dpp(v);
+    if constexpr (kWaves == 1) return v;
+    unsigned *r = red + turn * kWaves;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) r[(threadIdx.x / 64) % kWaves] = v;
+    __syncthreads();
+    unsigned s = 0u;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s = max(s, r[w]);
+    return s;
+  }
+};
+
+// The vector's elements c .. c+7, or `missing` where the caller has none.
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::type param8(const void *p, int c, int n, float missing) {
+  if (p) return load8(static_cast<const T *>(p), c, n);
+  typename Vec8<T>::type v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (T)missing;
+  return v;
+}
+
+// (v - mean) / deviation or v / rms of a row in place, elements behind the row's end 0; returns 1 / deviation.  Two
+// passes over the registers: the mean first, then the squares around it, so that a large mean costs no digits.
+template <int TPR, int NV>
+__device__ __forceinline__ float normalize(float (&v)[NV][8], int kind, float eps, int cols, int c0, RowReduce<TPR> &red) {
+  const float inv_n = 1.0f / (float)cols;
+  if (kind == SOUFFLE_NORM_LAYER) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += v[i][e];
+    const float mean = red.sum(s) * inv_n;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = c0 + i * TPR * 8 + e < cols ? v[i][e] - mean : 0.f;
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = __builtin_fmaf(v[i][e], v[i][e], s);
+  const float r = 1.0f / sqrtf(red.sum(s) * inv_n + eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] *= r;
+  return r;
+}
+
+template <class T, int TPR, int NV, int WG, bool OUT8>
+__global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
+  typedef typename Vec8<T>::type V;
+  constexpr int kSlots = WG / TPR;
+  __shared__ unsigned lds_red[WG / 64 * 2];
+  const int slot = threadIdx.x / TPR, t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
+  RowReduce<TPR> red{lds_red + slot * 2 * RowReduce<TPR>::kWaves, 0};
+
+  V pg[NV], pb[NV], gt[NV], ng[NV], nb[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = c0 + i * TPR * 8;
+    pg[i] = param8<T>(a.post_gamma, c, n, 1.f);
+    pb[i] = param8<T>(a.post_beta, c, n, 0.f);
+    ng[i] = param8<T>(a.pre_gamma, c, n, 1.f);
+    nb[i] = param8<T>(a.pre_beta, c, n, 0.f);
+    gt[i] = param8<T>(nullptr, c, n, 1.f);
+  }
+  const int first = (blockIdx.x * kSlots + slot) * a.rows_per_slot, end = min(first + a.rows_per_slot, a.rows);
+  int gate_row = -1;
+  V xv[NV], fv[NV];
+  auto fetch = [&](int row) {
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx, *f = static_cast<const T *>(a.f) + row * a.ldf;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      xv[i] = load8(x, c0 + i * TPR * 8, n);
+      fv[i] = load8(f, c0 + i * TPR * 8, n);
+    }
+  };
+  // (rows of several waves: one row per workgroup at a time, so every thread takes the same turns through the barriers)
+  if (first < end) fetch(first);
+  for (int row = first; row < end; ++row) {
+    if (a.gate) {
+      const int gr = row / a.rows_per_gate;
+      if (gr != gate_row) {
+        gate_row = gr;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) gt[i] = load8(static_cast<const T *>(a.gate) + (long long)gr * n, c0 + i * TPR * 8, n);
+      }
+    }
+    float x[NV][8], p[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      to_f32(x[i], xv[i]);
+      to_f32(p[i], fv[i]);
+    }
+    if (row + 1 < end) fetch(row + 1);
+    if (a.post != SOUFFLE_NORM_NONE) (void)normalize<TPR, NV>(p, a.post, a.post_eps, n, c0, red);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = __builtin_fmaf(p[i][e], (float)pg[i][e], (float)pb[i][e]);
+        x[i][e] = __builtin_fmaf((float)gt[i][e], v, a.a * x[i][e]);
+      }
+    if (a.y) {
+      T *y = static_cast<T *>(a.y) + row * a.ldy;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store8(y, c0 + i * TPR * 8, n, from_f32<T>(x[i]));
+    }
+    (void)normalize<TPR, NV>(x, a.pre, a.pre_eps, n, c0, red);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = __builtin_fmaf(x[i][e], (float)ng[i][e], (float)nb[i][e]);
+    if constexpr (!OUT8) {
+      T *h = static_cast<T *>(a.h) + row * a.ldh;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store8(h, c0 + i * TPR * 8, n, from_f32<T>(x[i]));
+    } else {
+      unsigned m = 0u;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c0 + i * TPR * 8 + e < n) m = max(m, abs_bits(x[i][e]));
+      const RowScale rs = row_scale(red.umax(m));
+      int8_t *q = a.q + row * a.ldq;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = c0 + i * TPR * 8;      // (a q row has room up to a multiple of 64)
+        if (c < n) *reinterpret_cast<u2 *>(q + c) = quantize8(x[i], rs);
+      }
+      if (t == 0) a.q_scale[row] = rs.scale;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ backward ----
+enum { kPreGamma = 0, kPreBeta, kGate, kPostGamma, kPostBeta, kVectors };
+
+struct BwdArgs {
+  const void *x, *f, *dy, *dh, *post_gamma, *post_beta, *gate, *pre_gamma;
+  void *dx, *df;                    // nullable
+  void *dgate;                      // written here where a group of rows is one workgroup's own
+  float *partial;                   // [chunks][wanted vectors][cols]
+  long long ldx, ldf, ld_dy, ld_dh, ld_dx, ld_df;
+  int rows, cols, post, pre;
+  int rows_per_gate;                // rows that share a gate row (all rows: one gate row, or no gate)
+  int chunk_rows;                   // rows of a workgroup; a multiple of rows_per_gate, or within one gate row's rows
+  int chunks_per_gate;              // > 0: that many chunks per gate row; 0: chunks hold whole gate rows
+  int vectors, wanted;              // wanted: bit v set = the gradient of vector v is collected
+  float a, post_eps, pre_eps;
+};
+
+// Several rows at a time (one per slot of TPR threads), slots in step, so that a barrier of the workgroup serves them all.
+template <class T, int TPR, int NV, int WG>
+__global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
+  typedef typename Vec8<T>::type V;
+  constexpr int kSlots = WG / TPR;
+  __shared__ unsigned lds_red[WG / 64 * 2];
+  __shared__ float lds_sum[kSlots > 1 ? TPR * NV * 8 : 1];
+  const int slot = threadIdx.x / TPR, t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
+  const float inv_n = 1.0f / (float)n;
+  RowReduce<TPR> red{lds_red + slot * 2 * RowReduce<TPR>::kWaves, 0};
+
+  float sums[kVectors][NV][8] = {};
+  // The slots' sums of vector v, added in the slots' order, to out[0 .. cols) by the first slot.
+  auto collect = [&](int v, auto store) {
+    if constexpr (kSlots > 1) {
+      for (int s = 1; s < kSlots; ++s) {
+        if (slot == s)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) lds_sum[(i * 8 + e) * TPR + t] = sums[v][i][e];
+        __syncthreads();
+        if (slot == 0)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sums[v][i][e] += lds_sum[(i * 8 + e) * TPR + t];
+        __syncthreads();
+      }
+    }
+    if (slot == 0)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store(c0 + i * TPR * 8, sums[v][i]);
+  };
+
+  int first, end;
+  if (a.chunks_per_gate > 0) {
+    const int g = blockIdx.x / a.chunks_per_gate, k = blockIdx.x % a.chunks_per_gate, g_end = min((g + 1) * a.rows_per_gate, a.rows);
+    first = min(g * a.rows_per_gate + k * a.chunk_rows, g_end);
+    end = min(first + a.chunk_rows, g_end);
+  } else {
+    first = min((long long)blockIdx.x * a.chunk_rows, (long long)a.rows);
+    end = min(first + a.chunk_rows, a.rows);
+  }
+  // rows first .. end in runs that share a gate row
+  for (int run = first; run < end;) {
+    const int gr = run / a.rows_per_gate, run_end = min((gr + 1) * a.rows_per_gate, end);
+    V gt[NV], pg[NV], pb[NV], ng[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = c0 + i * TPR * 8;
+      gt[i] = param8<T>(a.gate ? static_cast<const T *>(a.gate) + (long long)gr * n : nullptr, c, n, 1.f);
+      pg[i] = param8<T>(a.post_gamma, c, n, 1.f);
+      pb[i] = param8<T>(a.post_beta, c, n, 0.f);
+      ng[i] = param8<T>(a.pre_gamma, c, n, 1.f);
+    }
+    V xv[NV], fv[NV], yv[NV], hv[NV];
+    auto fetch = [&](int row) {      // (a slot without a row takes the run's first one, with gradients of zero)
+      const bool valid = row < run_end;
+      const long long r = valid ? row : run;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = c0 + i * TPR * 8, cd = valid ? c : n;
+        xv[i] = load8(static_cast<const T *>(a.x) + r * a.ldx, c, n);
+        fv[i] = load8(static_cast<const T *>(a.f) + r * a.ldf, c, n);
+        if (a.dy) yv[i] = load8(static_cast<const T *>(a.dy) + r * a.ld_dy, cd, n);
+        if (a.dh) hv[i] = load8(static_cast<const T *>(a.dh) + r * a.ld_dh, cd, n);
+      }
+    };
+    fetch(run + slot);
+    for (int base = run; base < run_end; base += kSlots) {
+      const int row = base + slot;
+      const bool valid = row < run_end;
+      float y[NV][8], fh[NV][8], d[NV][8], h[NV][8];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        to_f32(y[i], xv[i]);
+        to_f32(fh[i], fv[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[i][e] = a.dy ? (float)yv[i][e] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] = a.dh ? (float)hv[i][e] : 0.f;
+      }
+      if (base + kSlots < run_end) fetch(row + kSlots);
+      float fr = 1.f;
+      if (a.post != SOUFFLE_NORM_NONE) fr = normalize<TPR, NV>(fh, a.post, a.post_eps, n, c0, red);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          y[i][e] = __builtin_fmaf((float)gt[i][e], __builtin_fmaf(fh[i][e], (float)pg[i][e], (float)pb[i][e]), a.a * y[i][e]);
+      const float yr = normalize<TPR, NV>(y, a.pre, a.pre_eps, n, c0, red);
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sums[kPreGamma][i][e] = __builtin_fmaf(h[i][e], y[i][e], sums[kPreGamma][i][e]);
+          sums[kPreBeta][i][e] += h[i][e];
+          h[i][e] *= (float)ng[i][e];
+          s0 += h[i][e];
+          s1 = __builtin_fmaf(h[i][e], y[i][e], s1);
+        }
+      s0 = a.pre == SOUFFLE_NORM_LAYER ? red.sum(s0) * inv_n : 0.f;
+      s1 = red.sum(s1) * inv_n;
+      float s2 = 0.f, s3 = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          d[i][e] = __builtin_fmaf(yr, h[i][e] - s0 - y[i][e] * s1, d[i][e]);      // gradient of y
+          sums[kGate][i][e] = __builtin_fmaf(d[i][e], __builtin_fmaf(fh[i][e], (float)pg[i][e], (float)pb[i][e]), sums[kGate][i][e]);
+          y[i][e] = a.a * d[i][e];
+          d[i][e] *= (float)gt[i][e];                                              // gradient of N_post(f)
+          if (!(c0 + i * TPR * 8 + e < n && valid)) d[i][e] = 0.f;
+          sums[kPostGamma][i][e] = __builtin_fmaf(d[i][e], fh[i][e], sums[kPostGamma][i][e]);
+          sums[kPostBeta][i][e] += d[i][e];
+          d[i][e] *= (float)pg[i][e];
+          s2 += d[i][e];
+          s3 = __builtin_fmaf(d[i][e], fh[i][e], s3);
+        }
+      if (a.dx && valid)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store8(static_cast<T *>(a.dx) + row * a.ld_dx, c0 + i * TPR * 8, n, from_f32<T>(y[i]));
+      if (a.post != SOUFFLE_NORM_NONE) {
+        s2 = a.post == SOUFFLE_NORM_LAYER ? red.sum(s2) * inv_n : 0.f;
+        s3 = red.sum(s3) * inv_n;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[i][e] = fr * (d[i][e] - s2 - fh[i][e] * s3);
+      }
+      if (a.df && valid)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store8(static_cast<T *>(a.df) + row * a.ld_df, c0 + i * TPR * 8, n, from_f32<T>(d[i]));
+    }
+    if (a.dgate && a.chunks_per_gate == 0) {      // the gate row's rows were all this workgroup's
+      collect(kGate, [&](int c, const float (&v)[8]) { store8(static_cast<T *>(a.dgate) + (long long)gr * n, c, n, from_f32<T>(v)); });
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[kGate][i][e] = 0.f;
+    }
+    run = run_end;
+  }
+  float *out = a.partial + (long long)blockIdx.x * a.vectors * n;
+#pragma unroll
+  for (int v = 0; v < kVectors; ++v)
+    if (a.wanted >> v & 1) {
+      float *o = out + (long long)__popc(a.wanted & ((1 << v) - 1)) * n;
+      collect(v, [&](int c, const float (&s)[8]) { store8(o, c, n, from_f32<float>(s)); });
+    }
+}
+
+struct FinishArgs {
+  const float *partial;
+  void *out[kVectors];
+  int cols, vectors, wanted, chunks, chunks_per_gate;
+};
+// Column sums over the chunks: 64 columns x 16 slices of the chunks per workgroup, slices added in order.
+template <class T>
+__global__ void __launch_bounds__(1024) k_gated_norm_grad_finish(const FinishArgs a) {
+  __shared__ float lds[16][64];
+  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  int v = 0, seen = 0, first = 0, count = a.chunks;
+  long long row = 0;
+  // blockIdx.y: the wanted vectors in order, then the gate's further rows
+  int y = blockIdx.y;
+  if (y >= a.vectors) {
+    row = y - a.vectors + 1;
+    y = __popc(a.wanted & ((1 << kGate) - 1));
+  }
+  for (v = 0; v < kVectors; ++v)
+    if (a.wanted >> v & 1) {
+      if (seen == y) break;
+      ++seen;
+    }
+  if (v == kGate && a.chunks_per_gate > 0) {
+    first = (int)row * a.chunks_per_gate;
+    count = a.chunks_per_gate;
+  }
+  float s = 0.f;
+  if (c < a.cols) {
+    const float *p = a.partial + ((long long)first * a.vectors + y) * a.cols + c;
+#pragma unroll 4
+    for (int k = slice; k < count; k += 16) s += p[(long long)k * a.vectors * a.cols];
+  }
+  lds[slice][lane] = s;
+  __syncthreads();
+  if (slice == 0 && c < a.cols) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += lds[k][lane];
+    static_cast<T *>(a.out[v])[row * a.cols + c] = (T)s;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host side ----
+constexpr int kMaxCols = 16384;
+
+static int check_cfg(const souffle_gated_norm_cfg *c) {
+  if (!c) return fail(SOUFFLE_ERR_NULL, "cfg is NULL");
+  if (c->rows < 0) return fail(SOUFFLE_ERR_SHAPE, "rows must not be negative (got %d)", c->rows);
+  if (c->cols < 1 || c->cols > kMaxCols) return fail(SOUFFLE_ERR_SHAPE, "cols must be in 1..%d (got %d)", kMaxCols, c->cols);
+  if (c->dtype != SOUFFLE_F16 && c->dtype != SOUFFLE_BF16 && c->dtype != SOUFFLE_F32) return fail(SOUFFLE_ERR_SHAPE, "unknown dtype %d", c->dtype);
+  if (c->post_norm < SOUFFLE_NORM_NONE || c->post_norm > SOUFFLE_NORM_RMS) return fail(SOUFFLE_ERR_SHAPE, "unknown post_norm %d", c->post_norm);
+  if (c->pre_norm != SOUFFLE_NORM_LAYER && c->pre_norm != SOUFFLE_NORM_RMS) return fail(SOUFFLE_ERR_SHAPE, "pre_norm must be LAYER or RMS (got %d)", c->pre_norm);
+  if (c->rows_per_gate < 0 || (c->rows_per_gate > 0 && c->rows % c->rows_per_gate))
+    return fail(SOUFFLE_ERR_SHAPE, "rows_per_gate must divide the %d rows (got %d)", c->rows, c->rows_per_gate);
+  if (!(c->post_eps >= 0.f) || !(c->pre_eps >= 0.f)) return fail(SOUFFLE_ERR_SHAPE, "the norms' eps must not be negative");
+  return SOUFFLE_OK;
+}
+static int check_row(const char *name, const void *p, long long ld, const souffle_gated_norm_cfg *c) {
+  const unsigned size = c->dtype == SOUFFLE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(p) % size) return fail(SOUFFLE_ERR_ALIGN, "%s is not aligned to its elements", name);
+  if (ld < c->cols) return fail(SOUFFLE_ERR_SHAPE, "the rows of %s overlap: stride %lld, %d columns", name, ld, c->cols);
+  return SOUFFLE_OK;
+}
+static int check_vectors(const souffle_gated_norm_cfg *c, const souffle_gated_norm_w *w) {
+  if (!w) return fail(SOUFFLE_ERR_NULL, "the vectors' struct is NULL");
+  if (c->post_norm == SOUFFLE_NORM_NONE && (w->post_gamma || w->post_beta)) return fail(SOUFFLE_ERR_SHAPE, "post_gamma and post_beta need a post_norm");
+  const void *p[5] = {w->post_gamma, w->post_beta, w->gate, w->pre_gamma, w->pre_beta};
+  for (int i = 0; i < 5; ++i)
+    if (reinterpret_cast<uintptr_t>(p[i]) % (c->dtype == SOUFFLE_F32 ? 4 : 2)) return fail(SOUFFLE_ERR_ALIGN, "a vector is not aligned to its elements");
+  return SOUFFLE_OK;
+}
+
+template <class T, int TPR, int NV, int WG>
+static int launch_fwd(FwdArgs a, int num_cus, hipStream_t st) {
+  constexpr int kSlots = WG / TPR;
+  const long long slots = (long long)num_cus * (2048 / WG) * kSlots;      // row slots that are resident at once
+  a.rows_per_slot = (int)std::max<long long>(1, (a.rows + slots - 1) / slots);
+  const int grid = (int)(((long long)a.rows + (long long)a.rows_per_slot * kSlots - 1) / ((long long)a.rows_per_slot * kSlots));
+  if (a.q) hipLaunchKernelGGL((k_gated_norm<T, TPR, NV, WG, true>), dim3(grid), dim3(WG), 0, st, a);
+  else hipLaunchKernelGGL((k_gated_norm<T, TPR, NV, WG, false>), dim3(grid), dim3(WG), 0, st, a);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
+template <class T>
+static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
+  if (a.cols <= 512) return launch_fwd<T, 64, 1, 256>(a, num_cus, st);
+  if (a.cols <= 1024) return launch_fwd<T, 64, 2, 256>(a, num_cus, st);
+  if (a.cols <= 2048) return launch_fwd<T, 256, 1, 256>(a, num_cus, st);
+  if (a.cols <= 4096) return launch_fwd<T, 256, 2, 256>(a, num_cus, st);
+  if (a.cols <= 8192) return launch_fwd<T, 512, 2, 512>(a, num_cus, st);
+  return launch_fwd<T, 1024, 2, 1024>(a, num_cus, st);
+}
+
+// How the rows are cut into chunks, one workgroup each: about `want` of them, none across gate rows unless it holds
+// whole gate rows.
+struct Chunks {
+  int count, rows, per_gate;
+};
+static Chunks plan_chunks(int rows, int rows_per_gate, int gate_grad, int want) {
+  Chunks c;
+  if (!gate_grad) {
+    c.rows = std::max(1, (rows + want - 1) / want);
+    c.per_gate = 0;
+    c.count = (rows + c.rows - 1) / c.rows;
+    return c;
+  }
+  const int gates = rows / rows_per_gate;
+  if (gates >= want) {
+    const int per_chunk = (gates + want - 1) / want;
+    c.rows = per_chunk * rows_per_gate;
+    c.per_gate = 0;
+    c.count = (gates + per_chunk - 1) / per_chunk;
+  } else {
+    c.per_gate = std::max(1, std::min(rows_per_gate, want / gates));
+    c.rows = (rows_per_gate + c.per_gate - 1) / c.per_gate;
+    c.per_gate = (rows_per_gate + c.rows - 1) / c.rows;
+    c.count = c.per_gate * gates;
+  }
+  return c;
+}
+constexpr int kChunks = 256;      // one per CU
+
+static int wanted_vectors(const souffle_gated_norm_grad *g) {
+  return (g->pre_gamma ? 1 << kPreGamma : 0) | (g->pre_beta ? 1 << kPreBeta : 0) | (g->gate ? 1 << kGate : 0) |
+         (g->post_gamma ? 1 << kPostGamma : 0) | (g->post_beta ? 1 << kPostBeta : 0);
+}
+
+template <class T, int TPR, int NV, int WG>
+static int launch_bwd(const BwdArgs &a, int chunks, hipStream_t st) {
+  hipLaunchKernelGGL((k_gated_norm_grad<T, TPR, NV, WG>), dim3(chunks), dim3(WG), 0, st, a);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
+template <class T>
+static int backward(const BwdArgs &a, const FinishArgs &f, int gate_rows, hipStream_t st) {
+  int rc;
+  if (a.cols <= 512) rc = launch_bwd<T, 64, 1, 512>(a, f.chunks, st);
+  else if (a.cols <= 1024) rc = launch_bwd<T, 128, 1, 512>(a, f.chunks, st);
+  else if (a.cols <= 2048) rc = launch_bwd<T, 256, 1, 512>(a, f.chunks, st);
+  else if (a.cols <= 4096) rc = launch_bwd<T, 512, 1, 512>(a, f.chunks, st);
+  else if (a.cols <= 8192) rc = launch_bwd<T, 1024, 1, 1024>(a, f.chunks, st);
+  else rc = launch_bwd<T, 1024, 2, 1024>(a, f.chunks, st);
+  if (rc || f.vectors == 0) return rc;
+  const int more = (f.wanted >> kGate & 1) ? gate_rows - 1 : 0;
+  hipLaunchKernelGGL(k_gated_norm_grad_finish<T>, dim3((a.cols + 63) / 64, f.vectors + more), dim3(1024), 0, st, f);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
+
+static int run_forward(const souffle_gated_norm_cfg *c, const souffle_gated_norm_w *w, const void *x, const void *f, void *y, void *h,
+                       int8_t *q, long long ldq, float *q_scale, souffle_stream_t stream) {
+  if (int rc = check_cfg(c)) return rc;
+  if (int rc = check_vectors(c, w)) return rc;
+  if (c->rows == 0) return SOUFFLE_OK;
+  if (!x || !f) return fail(SOUFFLE_ERR_NULL, "x and f must not be NULL");
+  if (int rc = check_row("x", x, c->ldx, c)) return rc;
+  if (int rc = check_row("f", f, c->ldf, c)) return rc;
+  if (y)
+    if (int rc = check_row("y", y, c->ldy, c)) return rc;
+  if (h)
+    if (int rc = check_row("h", h, c->ldh, c)) return rc;
+  DeviceFacts df;
+  if (int rc = device_facts(&df)) return rc;
+  FwdArgs a = {x, f, w->post_gamma, w->post_beta, w->gate, w->pre_gamma, w->pre_beta, y, h, q, q_scale, c->ldx, c->ldf, c->ldy, c->ldh, ldq,
+               c->rows, c->cols, c->post_norm, c->pre_norm, c->rows_per_gate ? c->rows_per_gate : c->rows, 1, c->residual_scale, c->post_eps, c->pre_eps};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (c->dtype == SOUFFLE_F16) return forward<half_t>(a, df.num_cus, st);
+  if (c->dtype == SOUFFLE_BF16) return forward<bf16_t>(a, df.num_cus, st);
+  return forward<float>(a, df.num_cus, st);
+}
+
+}  // namespace gated_norm
+}  // namespace souffle
+
+using namespace souffle;
+using namespace souffle::gated_norm;
+
+extern "C" int souffle_gated_norm_forward(const souffle_gated_norm_cfg *cfg, const souffle_gated_norm_w *w, const void *x, const void *f,
+                                          void *y, void *h, souffle_stream_t stream) {
+  if (cfg && cfg->rows > 0 && !h) return fail(SOUFFLE_ERR_NULL, "h must not be NULL");
+  return run_forward(cfg, w, x, f, y, h, nullptr, 0, nullptr, stream);
+}
+
+extern "C" int souffle_gated_norm_forward_int8(const souffle_gated_norm_cfg *cfg, const souffle_gated_norm_w *w, const void *x, const void *f,
+                                               void *y, int8_t *q, long long ldq, float *row_scale, souffle_stream_t stream) {
+  if (cfg && cfg->rows > 0) {
+    if (!q || !row_scale) return fail(SOUFFLE_ERR_NULL, "q and row_scale must not be NULL");
+    if (!aligned16(q) || ldq % 16) return fail(SOUFFLE_ERR_ALIGN, "the rows of q must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(row_scale) % 4) return fail(SOUFFLE_ERR_ALIGN, "row_scale is not aligned to its elements");
+    if (ldq < (long long)round_up((size_t)std::max(cfg->cols, 0), 64)) return fail(SOUFFLE_ERR_SHAPE, "ldq must be at least cols rounded up to 64 (got %lld)", ldq);
+  }
+  return run_forward(cfg, w, x, f, y, nullptr, q, ldq, row_scale, stream);
+}
+
+extern "C" size_t souffle_gated_norm_backward_workspace_bytes(const souffle_gated_norm_cfg *cfg) {
+  if (check_cfg(cfg)) return 0;
+  // the most chunks that any set of wanted gradients makes, each with all five vectors
+  const int rpg = cfg->rows_per_gate ? cfg->rows_per_gate : std::max(cfg->rows, 1);
+  const int chunks = std::max(plan_chunks(cfg->rows, rpg, 0, kChunks).count, cfg->rows ? plan_chunks(cfg->rows, rpg, 1, kChunks).count : 0);
+  return round_up((size_t)std::max(chunks, 1) * kVectors * cfg->cols * 4, 256);
+}
+
+extern "C" int souffle_gated_norm_backward(const souffle_gated_norm_cfg *c, const souffle_gated_norm_w *w, const void *dy, const void *dh,
+                                           const void *x, const void *f, const souffle_gated_norm_grad *g, void *ws, size_t ws_bytes,
+                                           souffle_stream_t stream) {
+  if (int rc = check_cfg(c)) return rc;
+  if (int rc = check_vectors(c, w)) return rc;
+  if (!g) return fail(SOUFFLE_ERR_NULL, "the gradients' struct is NULL");
+  if (c->rows == 0) return fail(SOUFFLE_ERR_SHAPE, "there are no rows to take gradients of");
+  if (!x || !f || (!dy && !dh)) return fail(SOUFFLE_ERR_NULL, "x, f and one of dy and dh must not be NULL");
+  if (c->post_norm == SOUFFLE_NORM_NONE && (g->post_gamma || g->post_beta)) return fail(SOUFFLE_ERR_SHAPE, "gradients of post_gamma and post_beta need a post_norm");
+  if (g->gate && !w->gate) return fail(SOUFFLE_ERR_NULL, "the gate's gradient needs the gate");
+  const struct { const char *name; const void *p; long long ld; } rows[6] = {{"x", x, c->ldx}, {"f", f, c->ldf}, {"dy", dy, g->ld_dy}, {"dh", dh, g->ld_dh},
+                                                                            {"dx", g->dx, g->ld_dx}, {"df", g->df, g->ld_df}};
+  for (const auto &r : rows)
+    if (r.p)
+      if (int rc = check_row(r.name, r.p, r.ld, c)) return rc;
+  const void *vec[5] = {g->pre_gamma, g->pre_beta, g->gate, g->post_gamma, g->post_beta};
+  for (const void *p : vec)
+    if (reinterpret_cast<uintptr_t>(p) % (c->dtype == SOUFFLE_F32 ? 4 : 2)) return fail(SOUFFLE_ERR_ALIGN, "a gradient vector is not aligned to its elements");
+  const int rpg = c->rows_per_gate ? c->rows_per_gate : c->rows, wanted = wanted_vectors(g);
+  if (wanted) {
+    if (!ws || ws_bytes < souffle_gated_norm_backward_workspace_bytes(c))
+      return fail(SOUFFLE_ERR_WORKSPACE, "workspace too small: need %zu bytes", souffle_gated_norm_backward_workspace_bytes(c));
+    if (!aligned16(ws)) return fail(SOUFFLE_ERR_ALIGN, "workspace must be 16-byte aligned");
+  }
+  DeviceFacts df;
+  if (int rc = device_facts(&df)) return rc;
+  const Chunks ch = plan_chunks(c->rows, rpg, g->gate != nullptr, kChunks);
+  const bool gate_direct = g->gate && ch.per_gate == 0;
+  BwdArgs a = {};
+  a.x = x; a.f = f; a.dy = dy; a.dh = dh;
+  a.post_gamma = w->post_gamma; a.post_beta = w->post_beta; a.gate = w->gate; a.pre_gamma = w->pre_gamma;
+  a.dx = g->dx; a.df = g->df; a.dgate = gate_direct ? g->gate : nullptr;
+  a.partial = static_cast<float *>(ws);
+  a.ldx = c->ldx; a.ldf = c->ldf; a.ld_dy = g->ld_dy; a.ld_dh = g->ld_dh; a.ld_dx = g->ld_dx; a.ld_df = g->ld_df;
+  a.rows = c->rows; a.cols = c->cols; a.post = c->post_norm; a.pre = c->pre_norm;
+  a.rows_per_gate = rpg; a.chunk_rows = ch.rows; a.chunks_per_gate = ch.per_gate;
+  a.wanted = gate_direct ? wanted & ~(1 << kGate) : wanted;
+  a.vectors = __builtin_popcount(a.wanted);
+  a.a = c->residual_scale; a.post_eps = c->post_eps; a.pre_eps = c->pre_eps;
+  FinishArgs fin = {static_cast<const float *>(ws), {g->pre_gamma, g->pre_beta, g->gate, g->post_gamma, g->post_beta}, c->cols, a.vectors, a.wanted, ch.count, ch.per_gate};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int gate_rows = c->rows / rpg;
+  if (c->dtype == SOUFFLE_F16) return backward<half_t>(a, fin, gate_rows, st);
+  if (c->dtype == SOUFFLE_BF16) return backward<bf16_t>(a, fin, gate_rows, st);
+  return backward<float>(a, fin, gate_rows, st);
+}

@@ -1,0 +1,396 @@
+// Linear layers in 8-bit integers: rows quantised as they come (one scale per row), weights quantised once (one scale per
+// output channel), products on the integer matrix cores, scales, bias and activation in the epilogue.
+//
+//   q[m][k] = round_half_even(x[m][k] / s[m]),   y[m][n] = act(s[m] t[n] sum_k q[m][k] w[k][n] + b[n])
+//
+// The sums are 32-bit integers and exact (K <= 131071 keeps them in range), so neither the order of K nor a split of
+// it changes a result.
+//
+// Weights are kept in one packed copy [N/64][K/64][4 operands][64 lanes][16 bytes] (zeros up to multiples of 64): an
+// operand of v_mfma_i32_16x16x64_i8 is one contiguous KB that a wave loads straight into registers with one
+// 16-byte load per lane, and the four operands of 64 columns x 64 of K are 4 KB in a row.  Lane 16 c + 4 g + v of operand t holds
+// k = 16 c .. 16 c + 15 of column 16 g + 4 t + v.  With the weights as the instruction's first operand a lane's four
+// results are the columns 16 g + 4 t .. + 3 of one row (g = lane / 16), so over the four operands a lane owns 16 adjacent columns of a row: 32
+// bytes of an fp16 result.
+#include <algorithm>
+#include "typed.hpp"
+#include "host_util.hpp"
+
+namespace souffle {
+namespace linear_int8 {
+
+typedef int i4 __attribute__((ext_vector_type(4)));
+
+// v_mfma_i32_16x16x64_i8: D[i][j] += sum_k A[i][k] B[k][j]; lane l holds row i (column j) = l % 16, k = 16 (l / 16) .. + 15
+// of A (of B), and rows 4 (l / 16) .. + 3 of column l % 16 of D.
+__device__ __forceinline__ i4 mfma_i8(i4 a, i4 b, i4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ i4 ldg16(const int8_t *p) { return *(const __attribute__((address_space(1))) i4 *)p; }
+
+// ---------------------------------------------------------------------------------------- quantisation ----
+// Rows: TPR threads per row, NV vectors of 8 per thread kept in registers between the largest value and the rounding
+// (NV = 0: any length, the row is read again for the rounding).  Bound by memory: 3 bytes per fp16 element.
+template <class T, int TPR, int NV>
+__global__ void __launch_bounds__(256) k_quantize_rows(const T *x, long long ldx, int8_t *q, long long ldq, float *scale, int rows, int cols) {
+  constexpr int kSlots = 256 / TPR;
+  __shared__ unsigned lds_max[4];
+  const int slot = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const long long row = (long long)blockIdx.x * kSlots + slot;
+  if (TPR == 64 && row >= rows) return;      // (whole waves; with 256 threads per row every workgroup has a row)
+  const T *xr = x + row * ldx;
+  int8_t *qr = q + row * ldq;
+  typename Vec8<T>::type v[NV ? NV : 1];
+  unsigned m = 0u;
+  auto widen = [&](typename Vec8<T>::type w) {
+    float f[8];
+    to_f32(f, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = load8(xr, (i * TPR + t) * 8, cols);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) widen(v[i]);
+  } else {
+    for (int c = t * 8; c < cols; c += TPR * 8) widen(load8(xr, c, cols));
+  }
+  m = wave_umax_dpp(m);
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) lds_max[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = max(max(lds_max[0], lds_max[1]), max(lds_max[2], lds_max[3]));
+  }
+  const RowScale rs = row_scale(m);
+  auto put = [&](typename Vec8<T>::type w, int c) {
+    float f[8];
+    to_f32(f, w);
+    if (c < cols) *reinterpret_cast<u2 *>(qr + c) = quantize8(f, rs);
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) put(v[i], (i * TPR + t) * 8);
+  } else {
+    for (int c = t * 8; c < cols; c += TPR * 8) put(load8(xr, c, cols), c);
+  }
+  if (t == 0) scale[row] = rs.scale;
+}
+
+// Byte offset of weight (k, n) in the packed copy.
+__device__ __forceinline__ size_t packed_at(int k, int n, int kblocks) {
+  const int kk = k & 63, nn = n & 63;
+  const int lane = 16 * (kk >> 4) + 4 * (nn >> 4) + (nn & 3), t = (nn >> 2) & 3;
+  return (((size_t)(n >> 6) * kblocks + (k >> 6)) * 4 + t) * 1024 + lane * 16 + (kk & 15);
+}
+
+// Weights, once per model: a workgroup takes 64 columns; scale and rounding per column.  W = int8_t: packing alone.
+template <class W>
+__global__ void __launch_bounds__(256) k_pack_weight(const W *w, long long ldw, int8_t *packed, float *scale, int K, int N) {
+  __shared__ unsigned lds_max[4][64];
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, n = blockIdx.x * 64 + lane, kblocks = (K + 63) / 64;
+  RowScale rs = {1.f, 1.f, true};
+  if constexpr (sizeof(W) > 1) {
+    unsigned m = 0u;
+    for (int k = part; k < K; k += 4)
+      if (n < N) m = max(m, abs_bits((float)w[k * ldw + n]));
+    lds_max[part][lane] = m;
+    __syncthreads();
+    m = max(max(lds_max[0][lane], lds_max[1][lane]), max(lds_max[2][lane], lds_max[3][lane]));
+    rs = row_scale(m);
+    if (part == 0 && n < N) scale[n] = rs.scale;
+  }
+  for (int k = part * 16; k < kblocks * 64; k += 64) {      // 16 of K: one lane's 16 bytes
+    unsigned d[4] = {0u, 0u, 0u, 0u};
+    for (int b = 0; b < 16; ++b)
+      if (k + b < K && n < N) {
+        int v;
+        if constexpr (sizeof(W) > 1) v = quantize((float)w[(k + b) * ldw + n], rs);
+        else v = w[(k + b) * ldw + n];
+        d[b >> 2] |= ((unsigned)v & 255u) << (8 * (b & 3));
+      }
+    *reinterpret_cast<u4 *>(packed + packed_at(k, n, kblocks)) = u4{d[0], d[1], d[2], d[3]};
+  }
+}
+
+// -------------------------------------------------------------------------------------------- products ----
+struct Args {
+  const int8_t *q;
+  long long ldq;
+  const float *row_scale;
+  const int8_t *packed;
+  const float *col_scale;
+  const void *bias;              // of the output's type, nullable
+  void *y;
+  long long ldy;
+  int M, N, K, act;
+  int kblocks;                   // K / 64, rounded up
+  int col_tiles;                 // workgroups along N
+};
+
+// NaN stays NaN in all of them.  The tanh GELU in its logistic form v / (1 + exp(-2 u)), u = 0.79788456 (v + 0.044715 v^3): exact
+// in both tails (1 - 1 / (1 + exp 2u) would lose the negative one's digits) and right for infinities.
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == SOUFFLE_ACT_RELU) return v < 0.f ? 0.f : v;
+  if (act == SOUFFLE_ACT_GELU_TANH) {
+    constexpr float K1 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, K2 = K1 * 0.044715f;
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * __builtin_fmaf(v * v, K2, K1)));
+  }
+  if (act == SOUFFLE_ACT_GELU_ERF) return gelu_erf(v);
+  return v;
+}
+
+// Columns n .. n+3 of row m.
+template <class T>
+__device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s) {
+  if (m >= a.M || n >= a.N) return;
+  const float rs = a.row_scale[m];
+  T *y = static_cast<T *>(a.y) + m * a.ldy + n;
+  const T *bias = static_cast<const T *>(a.bias);
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  typedef T V4u __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  V4 out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c = min(n + e, a.N - 1);
+    const float v = ((float)s[e] * a.col_scale[c]) * rs + (bias ? (float)bias[c] : 0.f);
+    out[e] = (T)activate(v, a.act);
+  }
+  if (n + 4 <= a.N) {
+    *reinterpret_cast<V4u *>(y) = out;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) y[e] = out[e];
+  }
+}
+
+// Few rows: a workgroup of W waves computes 16 MF rows x 16 NF columns, its waves take turns at K in steps of 64 with both
+// operands straight from memory into registers (nothing is shared between waves, so nothing goes through LDS and
+// the loop has no barrier), and the W partial sums meet in LDS at the end.
+template <class T, int MF, int NF, int W, int U>
+__global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
+  static_assert(NF == 1 || NF == 4, "one operand, or the four of 64 columns");
+  __shared__ i4 lds[W][MF * NF][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = blockIdx.x % a.col_tiles, group = NF == 4 ? col : col >> 2, t0 = NF == 4 ? 0 : col & 3, m0 = blockIdx.x / a.col_tiles * 16 * MF;
+  i4 acc[MF][NF] = {};
+  const int8_t *wp = a.packed + ((size_t)group * a.kblocks * 4 + t0) * 1024 + lane * 16;
+  const int8_t *xp[MF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i) xp[i] = a.q + min(m0 + 16 * i + (lane & 15), a.M - 1) * a.ldq + 16 * (lane >> 4);
+  // U of the wave's steps at a time, the next U loaded while the present ones are multiplied.  A step behind K's end reads the
+  // last one's operands again, with the weights replaced by zeros.
+  i4 wv[U][NF], xv[U][MF];
+  auto fetch = [&](int kb) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = min(kb + u * W, a.kblocks - 1);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) wv[u][j] = ldg16(wp + (size_t)k * 4096 + j * 1024);
+#pragma unroll
+      for (int i = 0; i < MF; ++i) xv[u][i] = ldg16(xp[i] + k * 64);
+    }
+  };
+  fetch(wave);
+  for (int kb = wave; kb < a.kblocks; kb += U * W) {
+    i4 wn[U][NF], xn[U][MF];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < NF; ++j) wn[u][j] = kb + u * W < a.kblocks ? wv[u][j] : i4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < MF; ++i) xn[u][i] = xv[u][i];
+    }
+    if (kb + U * W < a.kblocks) fetch(kb + U * W);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = mfma_i8(wn[u][j], xn[u][i], acc[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < MF; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) lds[wave][i * NF + j][lane] = acc[i][j];
+  __syncthreads();
+  for (int u = threadIdx.x; u < MF * NF * 64; u += W * 64) {
+    const int tile = u >> 6, l = u & 63;
+    i4 s = lds[0][tile][l];
+#pragma unroll
+    for (int w = 1; w < W; ++w) s += lds[w][tile][l];
+    finish4<T>(a, m0 + 16 * (tile / NF) + (l & 15), group * 64 + 16 * (l >> 4) + 4 * (t0 + tile % NF), s);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- host side ----
+constexpr int kMaxK = 131071;      // 128 * 128 * K stays below 2^31
+
+static bool known_dtype(int t) { return t == SOUFFLE_F16 || t == SOUFFLE_BF16 || t == SOUFFLE_F32; }
+static unsigned size_of(int t) { return t == SOUFFLE_F32 ? 4 : 2; }
+
+static int check_kn(int K, int N) {
+  if (K < 1 || K > kMaxK) return fail(SOUFFLE_ERR_SHAPE, "K must be in 1..%d (got %d)", kMaxK, K);
+  if (N < 1 || N > (1 << 24)) return fail(SOUFFLE_ERR_SHAPE, "N must be in 1..2^24 (got %d)", N);
+  return SOUFFLE_OK;
+}
+static int check_q(const void *q, long long ldq, int K) {
+  if (!aligned16(q) || ldq % 16) return fail(SOUFFLE_ERR_ALIGN, "the rows of q must be 16-byte aligned");
+  if (ldq < (long long)round_up(K, 64)) return fail(SOUFFLE_ERR_SHAPE, "ldq must be at least K rounded up to 64 (got %lld)", ldq);
+  return SOUFFLE_OK;
+}
+static int check_x(const char *name, const void *x, int dtype, long long ld, int cols) {
+  if (reinterpret_cast<uintptr_t>(x) % size_of(dtype)) return fail(SOUFFLE_ERR_ALIGN, "%s is not aligned to its elements", name);
+  if (ld < cols) return fail(SOUFFLE_ERR_SHAPE, "the rows of %s overlap: stride %lld, %d columns", name, ld, cols);
+  return SOUFFLE_OK;
+}
+
+template <class T>
+static int quantize_rows(const void *xv, long long ldx, int8_t *q, long long ldq, float *scale, int M, int K, hipStream_t st) {
+  const T *x = static_cast<const T *>(xv);
+  const dim3 wide(M), narrow((M + 3) / 4), block(256);
+  if (K <= 512) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 1024) hipLaunchKernelGGL((k_quantize_rows<T, 64, 2>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 2048) hipLaunchKernelGGL((k_quantize_rows<T, 256, 1>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 4096) hipLaunchKernelGGL((k_quantize_rows<T, 256, 2>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 8192) hipLaunchKernelGGL((k_quantize_rows<T, 256, 4>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else hipLaunchKernelGGL((k_quantize_rows<T, 256, 0>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
+static int quantize_rows(const void *x, int dtype, long long ldx, int8_t *q, long long ldq, float *scale, int M, int K, hipStream_t st) {
+  if (dtype == SOUFFLE_F16) return quantize_rows<half_t>(x, ldx, q, ldq, scale, M, K, st);
+  if (dtype == SOUFFLE_BF16) return quantize_rows<bf16_t>(x, ldx, q, ldq, scale, M, K, st);
+  return quantize_rows<float>(x, ldx, q, ldq, scale, M, K, st);
+}
+
+template <class T, int MF, int NF, int W, int U>
+static int launch_split(Args a, hipStream_t st) {
+  a.col_tiles = (a.N + 63) / 64 * (4 / NF);
+  const long long grid = (long long)a.col_tiles * ((a.M + 16 * MF - 1) / (16 * MF));
+  if (grid > 0x7fffffff) return fail(SOUFFLE_ERR_SHAPE, "M = %d rows of N = %d are more tiles than one launch holds", a.M, a.N);
+  hipLaunchKernelGGL((k_gemm_split<T, MF, NF, W, U>), dim3((unsigned)grid), dim3(W * 64), 0, st, a);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
+template <class T>
+static int gemm(const Args &a, hipStream_t st) {
+  if (a.M <= 16) return launch_split<T, 1, 1, 8, 4>(a, st);
+  if (a.M <= 32) return launch_split<T, 2, 1, 8, 4>(a, st);
+  return launch_split<T, 4, 4, 4, 1>(a, st);
+}
+static int gemm(const Args &a, int dtype, hipStream_t st) {
+  if (dtype == SOUFFLE_F16) return gemm<half_t>(a, st);
+  if (dtype == SOUFFLE_BF16) return gemm<bf16_t>(a, st);
+  return gemm<float>(a, st);
+}
+
+static int check_product(const void *packed, const float *col_scale, const void *bias, int act, const void *y, int dtype, long long ldy, int M,
+                         int N, int K) {
+  if (M < 0) return fail(SOUFFLE_ERR_SHAPE, "M must not be negative (got %d)", M);
+  if (int rc = check_kn(K, N)) return rc;
+  if (!known_dtype(dtype)) return fail(SOUFFLE_ERR_SHAPE, "unknown dtype %d", dtype);
+  if (act != SOUFFLE_ACT_NONE && act != SOUFFLE_ACT_RELU && act != SOUFFLE_ACT_GELU_TANH && act != SOUFFLE_ACT_GELU_ERF)
+    return fail(SOUFFLE_ERR_SHAPE, "unknown activation %d", act);
+  if (M == 0) return SOUFFLE_OK;
+  if (!packed || !col_scale || !y) return fail(SOUFFLE_ERR_NULL, "packed, col_scale and y must not be NULL");
+  if (!aligned16(packed)) return fail(SOUFFLE_ERR_ALIGN, "packed must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(col_scale) % 4 || reinterpret_cast<uintptr_t>(bias) % size_of(dtype))
+    return fail(SOUFFLE_ERR_ALIGN, "col_scale or bias is not aligned to its elements");
+  return check_x("y", y, dtype, ldy, N);
+}
+
+}  // namespace linear_int8
+}  // namespace souffle
+
+using namespace souffle;
+using namespace souffle::linear_int8;
+
+extern "C" size_t souffle_int8_packed_bytes(int K, int N) {
+  if (check_kn(K, N)) return 0;
+  return round_up(K, 64) * round_up(N, 64);
+}
+
+extern "C" int souffle_int8_pack_weight(const int8_t *w, long long ldw, void *packed, int K, int N, souffle_stream_t stream) {
+  if (int rc = check_kn(K, N)) return rc;
+  if (!w || !packed) return fail(SOUFFLE_ERR_NULL, "w and packed must not be NULL");
+  if (!aligned16(packed)) return fail(SOUFFLE_ERR_ALIGN, "packed must be 16-byte aligned");
+  if (ldw < N) return fail(SOUFFLE_ERR_SHAPE, "the rows of w overlap: stride %lld, %d columns", ldw, N);
+  DeviceFacts df;
+  if (int rc = device_facts(&df)) return rc;
+  hipLaunchKernelGGL(k_pack_weight<int8_t>, dim3((N + 63) / 64), dim3(256), 0, static_cast<hipStream_t>(stream), w, ldw, static_cast<int8_t *>(packed),
+                     static_cast<float *>(nullptr), K, N);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
+
+extern "C" int souffle_int8_quantize_weight(const void *w, int dtype, long long ldw, void *packed, float *col_scale, int K, int N, souffle_stream_t stream) {
+  if (int rc = check_kn(K, N)) return rc;
+  if (!known_dtype(dtype)) return fail(SOUFFLE_ERR_SHAPE, "unknown dtype %d", dtype);
+  if (!w || !packed || !col_scale) return fail(SOUFFLE_ERR_NULL, "w, packed and col_scale must not be NULL");
+  if (!aligned16(packed) || reinterpret_cast<uintptr_t>(col_scale) % 4) return fail(SOUFFLE_ERR_ALIGN, "packed must be 16-byte aligned, col_scale to its elements");
+  if (int rc = check_x("w", w, dtype, ldw, N)) return rc;
+  DeviceFacts df;
+  if (int rc = device_facts(&df)) return rc;
+  const dim3 grid((N + 63) / 64), block(256);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int8_t *p = static_cast<int8_t *>(packed);
+  if (dtype == SOUFFLE_F16) hipLaunchKernelGGL(k_pack_weight<half_t>, grid, block, 0, st, static_cast<const half_t *>(w), ldw, p, col_scale, K, N);
+  else if (dtype == SOUFFLE_BF16) hipLaunchKernelGGL(k_pack_weight<bf16_t>, grid, block, 0, st, static_cast<const bf16_t *>(w), ldw, p, col_scale, K, N);
+  else hipLaunchKernelGGL(k_pack_weight<float>, grid, block, 0, st, static_cast<const float *>(w), ldw, p, col_scale, K, N);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
+
+extern "C" int souffle_quantize_rows(const void *x, int dtype, long long ldx, int8_t *q, long long ldq, float *row_scale, int M, int K,
+                                     souffle_stream_t stream) {
+  if (M < 0) return fail(SOUFFLE_ERR_SHAPE, "M must not be negative (got %d)", M);
+  if (int rc = check_kn(K, 1)) return rc;
+  if (!known_dtype(dtype)) return fail(SOUFFLE_ERR_SHAPE, "unknown dtype %d", dtype);
+  if (M == 0) return SOUFFLE_OK;
+  if (!x || !q || !row_scale) return fail(SOUFFLE_ERR_NULL, "x, q and row_scale must not be NULL");
+  if (int rc = check_x("x", x, dtype, ldx, K)) return rc;
+  if (int rc = check_q(q, ldq, K)) return rc;
+  if (reinterpret_cast<uintptr_t>(row_scale) % 4) return fail(SOUFFLE_ERR_ALIGN, "row_scale is not aligned to its elements");
+  DeviceFacts df;
+  if (int rc = device_facts(&df)) return rc;
+  return quantize_rows(x, dtype, ldx, q, ldq, row_scale, M, K, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int souffle_gemm_int8(const int8_t *q, long long ldq, const float *row_scale, const void *packed, const float *col_scale,
+                                 const void *bias, int act, void *y, int dtype, long long ldy, int M, int N, int K, souffle_stream_t stream) {
+  if (int rc = check_product(packed, col_scale, bias, act, y, dtype, ldy, M, N, K)) return rc;
+  if (M == 0) return SOUFFLE_OK;
+  if (!q || !row_scale) return fail(SOUFFLE_ERR_NULL, "q and row_scale must not be NULL");
+  if (int rc = check_q(q, ldq, K)) return rc;
+  if (reinterpret_cast<uintptr_t>(row_scale) % 4) return fail(SOUFFLE_ERR_ALIGN, "row_scale is not aligned to its elements");
+  DeviceFacts df;
+  if (int rc = device_facts(&df)) return rc;
+  const Args a = {q, ldq, row_scale, static_cast<const int8_t *>(packed), col_scale, bias, y, ldy, M, N, K, act, (K + 63) / 64, 0};
+  return gemm(a, dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t souffle_linear_int8_workspace_bytes(int M, int K) {
+  if (M < 0 || check_kn(K, 1)) return 0;
+  return round_up((size_t)M * round_up(K, 64) + (size_t)M * 4, 256);
+}
+
+extern "C" int souffle_linear_int8(const void *x, long long ldx, const void *packed, const float *col_scale, const void *bias, int act, void *y,
+                                   int dtype, long long ldy, int M, int N, int K, void *ws, size_t ws_bytes, souffle_stream_t stream) {
+  if (int rc = check_product(packed, col_scale, bias, act, y, dtype, ldy, M, N, K)) return rc;
+  if (M == 0) return SOUFFLE_OK;
+  if (!x) return fail(SOUFFLE_ERR_NULL, "x must not be NULL");
+  if (int rc = check_x("x", x, dtype, ldx, K)) return rc;
+  if (!ws || ws_bytes < souffle_linear_int8_workspace_bytes(M, K))
+    return fail(SOUFFLE_ERR_WORKSPACE, "workspace too small: need %zu bytes", souffle_linear_int8_workspace_bytes(M, K));
+  if (!aligned16(ws)) return fail(SOUFFLE_ERR_ALIGN, "workspace must be 16-byte aligned");
+  DeviceFacts df;
+  if (int rc = device_facts(&df)) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const long long ldq = (long long)round_up(K, 64);
+  int8_t *q = static_cast<int8_t *>(ws);
+  float *row_scale = reinterpret_cast<float *>(q + (size_t)M * ldq);
+  if (int rc = quantize_rows(x, dtype, ldx, q, ldq, row_scale, M, K, st)) return rc;
+  const Args a = {q, ldq, row_scale, static_cast<const int8_t *>(packed), col_scale, bias, y, ldy, M, N, K, act, (K + 63) / 64, 0};
+  return gemm(a, dtype, st);
+}

@@ -1,0 +1,122 @@
+// Activations of three element types (fp16, bf16, fp32) for kernels that compute in fp32: vectors of 8 elements that are
+// loaded and stored in 16-byte pieces wherever a row starts, their conversion, and wave reductions without LDS traffic.
+#pragma once
+#include "common.hpp"
+#include "../../include/souffle_hip.h"
+
+namespace souffle {
+
+typedef __bf16 bf16_t;
+
+template <class T>
+struct Vec8 {
+  typedef T type __attribute__((ext_vector_type(8)));
+  // Rows may start at any multiple of the element's size (an odd width, a slice): the unaligned form is one
+  // global_load_dwordx4 / global_store_dwordx4 all the same, the memory unit splits it where it crosses a line.
+  typedef T unaligned __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+
+// Elements c .. c+7 of a row of n; what lies behind the row's end reads as zero.
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::type load8(const T *row, int c, int n) {
+  typedef typename Vec8<T>::type V;
+  if (c + 8 <= n) return *(const __attribute__((address_space(1))) typename Vec8<T>::unaligned *)(row + c);
+  V v = {};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (c + e < n) v[e] = *(const __attribute__((address_space(1))) T *)(row + c + e);
+  return v;
+}
+template <class T>
+__device__ __forceinline__ void store8(T *row, int c, int n, typename Vec8<T>::type v) {
+  if (c + 8 <= n) {
+    *(__attribute__((address_space(1))) typename Vec8<T>::unaligned *)(row + c) = v;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (c + e < n) *(__attribute__((address_space(1))) T *)(row + c + e) = v[e];
+}
+template <class V>
+__device__ __forceinline__ void to_f32(float (&f)[8], V v) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = (float)v[e];
+}
+// One rounding to nearest even per element (the compiler's conversions; fp32 passes through).
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::type from_f32(const float (&f)[8]) {
+  typename Vec8<T>::type v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (T)f[e];
+  return v;
+}
+
+// Reductions over the 64 lanes by DPP moves inside the vector unit (rows of 16, then across the rows); the result is
+// the same in every lane.  A shuffle goes through the LDS unit instead, at some 60 cycles a step, six steps a reduction.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float v, float identity) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, identity), __builtin_bit_cast(int, v), CTRL, ROWS, 15, false));
+}
+__device__ __forceinline__ float lane63(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+__device__ __forceinline__ float wave_sum_dpp(float v) {
+  v += dpp<0x111, 15>(v, 0.f);      // row_shr:1
+  v += dpp<0x112, 15>(v, 0.f);      // row_shr:2
+  v += dpp<0x114, 15>(v, 0.f);      // row_shr:4
+  v += dpp<0x118, 15>(v, 0.f);      // row_shr:8: lane 15 of each row of 16 holds the row's sum
+  v += dpp<0x142, 10>(v, 0.f);      // row_bcast:15 into rows 1 and 3
+  v += dpp<0x143, 12>(v, 0.f);      // row_bcast:31 into rows 2 and 3
+  return lane63(v);
+}
+// Largest of non-negative floats or NaNs, as bit patterns: NaN > infinity > finite, so a NaN is never lost.
+__device__ __forceinline__ unsigned wave_umax_dpp(unsigned v) {
+#define SOUFFLE_STEP(CTRL, ROWS) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 15, false))
+  SOUFFLE_STEP(0x111, 15);
+  SOUFFLE_STEP(0x112, 15);
+  SOUFFLE_STEP(0x114, 15);
+  SOUFFLE_STEP(0x118, 15);
+  SOUFFLE_STEP(0x142, 10);
+  SOUFFLE_STEP(0x143, 12);
+#undef SOUFFLE_STEP
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// ------------------------------------------------------------------ rows of 8-bit integers ----
+// A row x is held as q = round_half_even(x / s), s = max(fp32(max|x| / 127), 2^-100): |q| <= 127, and the bound keeps
+// 1 / s finite.  A row that holds a NaN or an infinity gets q = 0 and s = NaN, so that everything computed from it is NaN.
+struct RowScale {
+  float scale, inverse;
+  bool finite;
+};
+__device__ __forceinline__ unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+__device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
+  RowScale r;
+  r.finite = amax_bits < 0x7f800000u;
+  const float s = fmaxf(__builtin_bit_cast(float, amax_bits) / 127.0f, 0x1p-100f);
+  r.scale = r.finite ? s : __builtin_nanf("");
+  r.inverse = r.finite ? 1.0f / s : 0.0f;
+  return r;
+}
+// The rounding is that of the real quotient, not of a rounded one: halves are common (any value that is half its row's
+// largest is 63.5 s), and a product in fp32 would fall on either side of them.  t = x * (1/s) is off by less than 2^-16, so q0 = rint(t)
+// is right unless t lies within that of a half; there e = x - q0 s decides, which the fused multiply-add gives exactly
+// (x and q0 s are multiples of a power of two that |e| <= s holds fewer than 2^24 of).
+__device__ __forceinline__ int quantize(float x, const RowScale &r) {
+  const float t = x * r.inverse;
+  float q = __builtin_rintf(t);
+  if (__builtin_fabsf(t - q) > 0.4998f) {
+    const float e = __builtin_fmaf(-q, r.scale, x), half = 0.5f * r.scale;
+    if (e > half || (e == half && ((int)q & 1))) q += 1.0f;
+    else if (e < -half || (e == -half && ((int)q & 1))) q -= 1.0f;
+  }
+  return r.finite ? (int)q : 0;
+}
+__device__ __forceinline__ u2 quantize8(const float (&f)[8], const RowScale &r) {
+  u2 p = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) p[e >> 2] |= ((unsigned)quantize(f[e], r) & 255u) << (8 * (e & 3));
+  return p;
+}
+
+}  // namespace souffle

@@ -11,7 +11,9 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SOUFFLE_HIP_LIB") or os.path.join(_HERE, "libsouffle_hip.so")
 
-ACT_GELU_TANH, ACT_RELU, ACT_GELU_ERF = 0, 1, 2
+ACT_GELU_TANH, ACT_RELU, ACT_GELU_ERF, ACT_NONE = 0, 1, 2, 3
+F16, BF16, F32 = 0, 1, 2
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 GATES_IFGO, GATES_IGFO = 0, 1
 SE_MUL, SE_ADD = 0, 1
 
@@ -61,6 +63,21 @@ MB_NONE, MB_SWISH = 0, 1
 
 class MbconvBlock(C.Structure):
     _fields_ = [(n, C.c_int) for n in MB_INT_FIELDS] + [(n, C.c_void_p) for n in MB_PTR_FIELDS]
+
+
+class GatedNormCfg(C.Structure):
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("dtype", C.c_int), ("post_norm", C.c_int), ("pre_norm", C.c_int),
+                ("rows_per_gate", C.c_int), ("residual_scale", C.c_float), ("post_eps", C.c_float), ("pre_eps", C.c_float),
+                ("ldx", C.c_longlong), ("ldf", C.c_longlong), ("ldy", C.c_longlong), ("ldh", C.c_longlong)]
+
+
+class GatedNormW(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ["post_gamma", "post_beta", "gate", "pre_gamma", "pre_beta"]]
+
+
+class GatedNormGrad(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ["dx", "df", "pre_gamma", "pre_beta", "gate", "post_gamma", "post_beta"]] + \
+               [(n, C.c_longlong) for n in ["ld_dy", "ld_dh", "ld_dx", "ld_df"]]
 
 
 class DevInfo(C.Structure):
@@ -129,6 +146,23 @@ SIGNATURES = {
                                               C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "souffle_depthwise_conv2d_bn_swish": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                                     C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "souffle_int8_packed_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "souffle_int8_pack_weight": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "souffle_int8_quantize_weight": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "souffle_quantize_rows": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_int,
+                                        C.c_void_p]),
+    "souffle_gemm_int8": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                    C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "souffle_linear_int8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "souffle_linear_int8": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                      C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "souffle_gated_norm_forward": (C.c_int, [C.POINTER(GatedNormCfg), C.POINTER(GatedNormW), C.c_void_p, C.c_void_p, C.c_void_p,
+                                             C.c_void_p, C.c_void_p]),
+    "souffle_gated_norm_forward_int8": (C.c_int, [C.POINTER(GatedNormCfg), C.POINTER(GatedNormW), C.c_void_p, C.c_void_p, C.c_void_p,
+                                                  C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p]),
+    "souffle_gated_norm_backward_workspace_bytes": (C.c_size_t, [C.POINTER(GatedNormCfg)]),
+    "souffle_gated_norm_backward": (C.c_int, [C.POINTER(GatedNormCfg), C.POINTER(GatedNormW), C.c_void_p, C.c_void_p, C.c_void_p,
+                                              C.c_void_p, C.POINTER(GatedNormGrad), C.c_void_p, C.c_size_t, C.c_void_p]),
     "souffle_bench_us": (C.c_int, [BENCH_FN, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                    C.POINTER(C.c_double), C.POINTER(C.c_double)]),
 }

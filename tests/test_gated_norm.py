@@ -1,0 +1,396 @@
+"""The gated norm: forward, 8-bit rows and gradients against 64 bits with counted roundings, gradients against
+differences, refusals; and a block of gated norms and 8-bit linear layers as they are used together."""
+import ctypes as C
+
+import pytest
+import torch
+
+import norm_int8_ref as ref
+import souffle_hip as sh
+from gpu_util import announce
+
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+gpu = pytest.mark.gpu
+
+
+def values(seed, *shape, dtype=torch.float32, std=1.0, mean=0.0):
+    return (mean + std * torch.randn(*shape, generator=torch.Generator().manual_seed(seed))).to(dtype)
+
+
+def params(seed, rows, cols, dtype, post, pre, gate, affine=True):
+    """Keywords of the operator, tensors on the CPU.  gate: None, "channel", or a number of gate rows."""
+    p = {"residual_scale": 0.75, "post_norm": post, "pre_norm": pre, "post_eps": 1e-5, "pre_eps": 1e-6}
+    vec = lambda i, mean, *shape: values(seed + i, *shape, dtype=dtype, std=0.3, mean=mean)  # noqa: E731
+    if affine and post:
+        p["post_gamma"], p["post_beta"] = vec(1, 1.0, cols), vec(2, 0.0, cols)
+    if affine:
+        p["pre_gamma"], p["pre_beta"] = vec(3, 1.0, cols), vec(4, 0.0, cols)
+    if gate:
+        p["gate"] = vec(5, 0.5, cols) if gate == "channel" else vec(5, 0.5, gate, cols)
+    return p
+
+
+def cuda(p):
+    return {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in p.items()}
+
+
+def run_forward(x, f, p):
+    import gated_norm_binding as gn
+    t = x.dtype
+    y, h = gn.gated_norm(x.cuda(), f.cuda(), **cuda(p))
+    ry, rh, ey, eh = ref.forward(x, f, p)
+    ref.check("y", y, ry, ey + ref.half_step(ry, t))
+    ref.check("h", h, rh, eh + ref.half_step(rh, t))
+    y8, q, s = gn.gated_norm_int8(x.cuda(), f.cuda(), **cuda(p))
+    assert torch.equal(y8, y) and q.shape == h.shape
+    s, amax = s.double().cpu(), rh.abs().amax(-1)
+    assert ((s * 127 - amax).abs() <= eh.amax(-1) + 2 * ref.EPS32 * amax + 2.0 ** -93).all()
+    # rounded to the nearest step: half of one, what h may be off, and the quotient's last digit
+    assert ((q.double().cpu() * s[:, None] - rh).abs() <= 0.5 * s[:, None] * (1 + 2.0 ** -20) + eh).all()
+
+
+def run_backward(dy, dh, x, f, p):
+    import gated_norm_binding as gn
+    c = lambda v: None if v is None else v.cuda()  # noqa: E731
+    got = gn.gated_norm_backward(c(dy), c(dh), x.cuda(), f.cuda(), **cuda(p))
+    again = gn.gated_norm_backward(c(dy), c(dh), x.cuda(), f.cuda(), **cuda(p))
+    grads, bounds = ref.backward(dy, dh, x, f, p)
+    for name in ("x", "f", "gate", "post_gamma", "post_beta", "pre_gamma", "pre_beta"):
+        if name not in ("x", "f") and p.get(name) is None:
+            assert got[name] is None, name
+            continue
+        assert got[name].dtype == x.dtype
+        ref.check("gradient of " + name, got[name], grads[name], bounds[name] + ref.half_step(grads[name], x.dtype))
+        assert torch.equal(got[name], again[name]), "two calls differ: " + name
+    return got
+
+
+# ------------------------------------------------------------------------------------------------- CPU ----
+@pytest.mark.parametrize("post,pre,gate", [("layer", "layer", "channel"), ("rms", "rms", 3), (None, "layer", 2), ("layer", "rms", None)])
+def test_reference_gradients_are_those_of_automatic_differentiation(post, pre, gate):
+    x, f, dy, dh = (values(i, 6, 10, dtype=torch.float64) for i in range(4))
+    p = params(7, 6, 10, torch.float64, post, pre, gate)
+    leaves = {k: v.clone().requires_grad_(True) for k, v in {"x": x, "f": f, **p}.items() if isinstance(v, torch.Tensor)}
+    po = ref.norm(leaves["f"], post, 1e-5, leaves.get("post_gamma"), leaves.get("post_beta"))[0]
+    g = ref.gate_rows(leaves.get("gate"), 6)
+    y = 0.75 * leaves["x"] + (po if g is None else g * po)
+    h = ref.norm(y, pre, 1e-6, leaves.get("pre_gamma"), leaves.get("pre_beta"))[0]
+    auto = dict(zip(leaves, torch.autograd.grad([y, h], list(leaves.values()), [dy, dh])))
+    grads, bounds = ref.backward(dy, dh, x, f, p)
+    for name, v in auto.items():
+        assert (v - grads[name]).abs().max() < 1e-12, name
+        assert (bounds[name] < 1e-3 * (1 + grads[name].abs())).all(), "the bound of %s says nothing" % name
+
+
+def cfg(**k):
+    return sh.GatedNormCfg(*{**dict(rows=4, cols=32, dtype=0, post=1, pre=1, rpg=0, a=1.0, e1=1e-5, e2=1e-5, ldx=32, ldf=32, ldy=32, ldh=32), **k}.values())
+
+
+def test_refusals_without_gpu():
+    lib, P = sh.lib(), 4096
+    w = sh.GatedNormW()
+    fw = lambda c, w=w, x=P, f=P, y=P, h=P: lib.souffle_gated_norm_forward(C.byref(c), C.byref(w), x, f, y, h, None)  # noqa: E731
+    for bad in (dict(rows=-1), dict(cols=0), dict(cols=16385), dict(dtype=3), dict(post=3), dict(pre=0), dict(rpg=3), dict(rpg=-1), dict(e1=-1.0),
+                dict(e2=float("nan")), dict(ldx=31), dict(ldf=31), dict(ldy=31), dict(ldh=31)):
+        assert fw(cfg(**bad)) == -2, bad
+        assert sh.last_error()
+    assert lib.souffle_gated_norm_forward(None, C.byref(w), P, P, P, P, None) == -1
+    assert lib.souffle_gated_norm_forward(C.byref(cfg()), None, P, P, P, P, None) == -1
+    assert fw(cfg(), x=None) == -1 and fw(cfg(), f=None) == -1 and fw(cfg(), h=None) == -1
+    assert fw(cfg(), x=P + 1) == -3 and fw(cfg(dtype=2), h=P + 2) == -3 and fw(cfg(rows=0), x=None, f=None, y=None, h=None) == 0
+    assert fw(cfg(post=0), w=sh.GatedNormW(post_gamma=P)) == -2 and fw(cfg(), w=sh.GatedNormW(gate=P + 1)) == -3
+    f8 = lambda c, q=P, ldq=64, s=P: lib.souffle_gated_norm_forward_int8(C.byref(c), C.byref(w), P, P, None, q, ldq, s, None)  # noqa: E731
+    assert f8(cfg(), q=None) == -1 and f8(cfg(), s=None) == -1 and f8(cfg(), ldq=48) == -2 and f8(cfg(), ldq=72) == -3 and f8(cfg(), q=P + 8) == -3
+    n = lib.souffle_gated_norm_backward_workspace_bytes(C.byref(cfg()))
+    assert n >= 4 * 5 * 32 * 4 and lib.souffle_gated_norm_backward_workspace_bytes(C.byref(cfg(cols=0))) == 0
+    full = dict(dx=P, df=P, pre_gamma=P, pre_beta=P, gate=None, post_gamma=P, post_beta=P, ld_dy=32, ld_dh=32, ld_dx=32, ld_df=32)
+    bw = lambda c=cfg(), w=w, dy=P, dh=P, x=P, ws=P, n=n, **k: lib.souffle_gated_norm_backward(C.byref(c), C.byref(w), dy, dh, x, P, C.byref(sh.GatedNormGrad(**{**full, **k})), ws, n, None)  # noqa: E731
+    assert bw(dy=None, dh=None) == -1 and bw(x=None) == -1 and bw(gate=P) == -1
+    assert bw(ws=None) == -4 and bw(n=n - 1) == -4 and bw(ws=P + 8) == -3
+    assert bw(ld_dy=31) == -2 and bw(ld_dx=31) == -2 and bw(c=cfg(rows=0)) == -2 and bw(c=cfg(post=0)) == -2 and bw(df=P + 1) == -3 and bw(pre_beta=P + 1) == -3
+
+
+def test_bindings_refuse_cpu_tensors():
+    import gated_norm_binding as gn
+    z = torch.zeros(2, 8)
+    for call in (lambda: gn.gated_norm(z, z), lambda: gn.gated_norm_int8(z, z), lambda: gn.gated_norm_backward(z, z, z, z)):
+        with pytest.raises(TypeError, match="CUDA"):
+            call()
+
+
+# ------------------------------------------------------------------------------------------------- GPU ----
+@gpu
+def test_bindings_refuse_wrong_tensors():
+    announce("gated norm: refusals of the bindings")
+    import gated_norm_binding as gn
+    x = torch.zeros(6, 32, device="cuda")
+    v = torch.zeros(32, device="cuda")
+    bad = [(ValueError, (x, x[:5]), {}), (TypeError, (x, x.half()), {}), (TypeError, (x.double(), x.double()), {}), (ValueError, (x, x), dict(post_norm="batch")),
+           (ValueError, (x, x), dict(pre_norm=None)), (ValueError, (x, x), dict(gate=v[:31])), (ValueError, (x, x), dict(gate=torch.zeros(4, 32, device="cuda"))),
+           (ValueError, (x, x), dict(gate=v.half())), (ValueError, (x, x), dict(pre_gamma=v.view(1, 32))), (ValueError, (x, x), dict(post_norm=None, post_gamma=v)),
+           (ValueError, (x.t(), x.t()), {}), (ValueError, (x[:1].expand(6, 32), x), {}), (TypeError, (x, x), dict(gate=v.cpu())), (sh.SouffleError, (x, x), dict(pre_eps=-1.0))]
+    for error, args, kw in bad:
+        with pytest.raises(error):
+            gn.gated_norm(*args, **kw)
+    for dy, dh in ((None, None), (x[:5], x), (x, x.half())):
+        with pytest.raises(ValueError):
+            gn.gated_norm_backward(dy, dh, x, x)
+
+
+SIZES = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 513), (7, 768), (4, 1001), (3, 2048), (2, 2049), (3, 4096), (2, 4099), (2, 8192), (1, 8200), (2, 16384)]
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_forward_sizes(dtype, rows, cols):
+    announce("gated norm %s %dx%d" % (dtype, rows, cols))
+    x, f = values(1, rows, cols, dtype=TYPES[dtype], std=2.0), values(2, rows, cols, dtype=TYPES[dtype])
+    run_forward(x, f, params(3, rows, cols, TYPES[dtype], "layer", "layer", "channel"))
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_sizes(dtype, rows, cols):
+    announce("gated norm gradient %s %dx%d" % (dtype, rows, cols))
+    x, f, dy, dh = (values(i, rows, cols, dtype=TYPES[dtype]) for i in range(4))
+    run_backward(dy, dh, x, f, params(5, rows, cols, TYPES[dtype], "layer", "layer", "channel"))
+
+
+@gpu
+@pytest.mark.parametrize("post", ["layer", "rms", None])
+@pytest.mark.parametrize("pre", ["layer", "rms"])
+@pytest.mark.parametrize("gate", [None, "channel", 3, 12])
+@pytest.mark.parametrize("affine", [True, False])
+def test_every_form(post, pre, gate, affine):
+    announce("gated norm post=%s pre=%s gate=%s affine=%s" % (post, pre, gate, affine))
+    for dtype, cols in (("f32", 200), ("bf16", 1100)):
+        t = TYPES[dtype]
+        x, f, dy, dh = (values(10 + i, 12, cols, dtype=t, mean=0.2) for i in range(4))
+        p = params(9, 12, cols, t, post, pre, gate, affine)
+        run_forward(x, f, p)
+        run_backward(dy, dh, x, f, p)
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols,gate", [(700, 96, "channel"), (1111, 520, None), (600, 64, 300), (600, 64, 600), (260, 1032, 4), (515, 256, 5), (300, 4096, 2), (9000, 40, 9)])
+def test_many_rows(rows, cols, gate):
+    """Chunks of rows: inside one gate row, across several, as many gate rows as rows."""
+    announce("gated norm %dx%d gate=%s" % (rows, cols, gate))
+    x, f, dy, dh = (values(i, rows, cols) for i in range(4))
+    p = params(5, rows, cols, torch.float32, "layer", "rms", gate)
+    run_forward(x, f, p)
+    run_backward(dy, dh, x, f, p)
+
+
+@gpu
+def test_one_incoming_gradient():
+    announce("gated norm gradient: dy or dh alone")
+    x, f, d = (values(i, 20, 72) for i in range(3))
+    p = params(5, 20, 72, torch.float32, "rms", "layer", 4)
+    run_backward(d, None, x, f, p)
+    run_backward(None, d, x, f, p)
+
+
+@gpu
+@pytest.mark.parametrize("post,pre,gate", [("layer", "layer", "channel"), ("rms", "rms", 3), (None, "layer", 3), ("layer", "rms", None)])
+def test_gradients_against_differences(post, pre, gate):
+    """The change of sum(dy y + dh h) along a random direction of every input, by central differences in 64 bits: with
+    steps of 1e-4 they are good to 1e-7, the gradients in fp32 to 1e-5 of the terms' size (here about one per element)."""
+    announce("gated norm gradient against differences: %s %s %s" % (post, pre, gate))
+    import gated_norm_binding as gn
+    rows, cols = 6, 50
+    x, f, dy, dh = (values(20 + i, rows, cols) for i in range(4))
+    p = params(30, rows, cols, torch.float32, post, pre, gate)
+    got = gn.gated_norm_backward(dy.cuda(), dh.cuda(), x.cuda(), f.cuda(), **cuda(p))
+    inputs = {"x": x, "f": f, **{k: v for k, v in p.items() if isinstance(v, torch.Tensor)}}
+
+    def loss(inputs):
+        y, h, _, _ = ref.forward(inputs["x"], inputs["f"], {**p, **{k: v for k, v in inputs.items() if k not in ("x", "f")}})
+        return float((dy.double() * y + dh.double() * h).sum())
+    for i, (name, v) in enumerate(inputs.items()):
+        u = values(40 + i, *v.shape, dtype=torch.float64)
+        at = lambda e: loss({**inputs, name: v.double() + e * u})  # noqa: E731
+        diff = (at(1e-4) - at(-1e-4)) / 2e-4
+        along = float((got[name].double().cpu() * u).sum())
+        size = float((got[name].double().cpu() * u).abs().sum())
+        assert abs(diff - along) <= 1e-5 * size + 1e-6, (name, diff, along)
+
+
+@gpu
+def test_rows_apart_in_place_and_what_lies_around():
+    """Slices of wider tensors that start anywhere as inputs; through the C ABI: y over x and h over f in place, outputs in
+    rows apart, columns and rows around them left as they were."""
+    announce("gated norm: strides, in place, canaries")
+    import gated_norm_binding as gn
+    for t in TYPES.values():
+        for rows, cols in ((5, 77), (3, 1500)):
+            wide = [values(i, rows + 2, cols + 9, dtype=t).cuda() for i in range(2)]
+            x, f = (w[1:rows + 1, 3:cols + 3] for w in wide)
+            p = cuda(params(5, rows, cols, t, "layer", "rms", "channel"))
+            y0, h0 = gn.gated_norm(x.contiguous(), f.contiguous(), **p)
+            y1, h1 = gn.gated_norm(x, f, **p)
+            assert torch.equal(y0, y1) and torch.equal(h0, h1)
+            y2, h2 = gn.gated_norm(x, f, **p, want_y=False)
+            assert y2 is None and torch.equal(h0, h2)
+            d = values(8, rows, cols, dtype=t).cuda()
+            for a, b in zip(gn.gated_norm_backward(d, y0, x, f, **p).values(), gn.gated_norm_backward(d, y0, x.contiguous(), f.contiguous(), **p).values()):
+                assert (a is None and b is None) or torch.equal(a, b)
+            before = [w.clone() for w in wide]
+            c = sh.GatedNormCfg(rows, cols, {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}[t], 1, 2, 0, p["residual_scale"], p["post_eps"], p["pre_eps"],
+                                cols + 9, cols + 9, cols + 9, cols + 9)
+            w = sh.GatedNormW(*(sh.ptr(p.get(n)) for n in ("post_gamma", "post_beta", "gate", "pre_gamma", "pre_beta")))
+            sh.check(sh.lib().souffle_gated_norm_forward(C.byref(c), C.byref(w), x.data_ptr(), f.data_ptr(), x.data_ptr(), f.data_ptr(), sh.current_stream()))
+            torch.cuda.synchronize()
+            assert torch.equal(x, y0) and torch.equal(f, h0)
+            for now, old, inner in zip(wide, before, (y0, h0)):
+                old[1:rows + 1, 3:cols + 3] = inner
+                assert torch.equal(now, old), "written outside the rows"
+
+
+@gpu
+def test_hard_rows():
+    """Constant rows, zero rows, a mean a thousand times the deviation; NaN and infinity stay in their rows."""
+    announce("gated norm: constant, shifted and non-finite rows")
+    import gated_norm_binding as gn
+    x, f = values(1, 6, 300), values(2, 6, 300)
+    x[0], f[0] = 0, 0
+    x[1], f[1] = 3.0, -2.0
+    x[2] += 1000
+    f[2] += 1000
+    p = params(3, 6, 300, torch.float32, "layer", "layer", "channel")
+    run_forward(x, f, p)
+    run_backward(values(4, 6, 300), values(5, 6, 300), x, f, p)
+    y0, h0 = gn.gated_norm(x.cuda(), f.cuda(), **cuda(p))
+    x[3, 7], f[4, 299] = float("nan"), float("inf")
+    y, h = gn.gated_norm(x.cuda(), f.cuda(), **cuda(p))
+    _, q, s = gn.gated_norm_int8(x.cuda(), f.cuda(), **cuda(p))
+    assert torch.isnan(h[3]).all() and torch.isnan(h[4]).all() and torch.isnan(s[3:5]).all() and not q[3:5].any()
+    keep = [0, 1, 2, 5]
+    assert torch.equal(y[keep], y0[keep]) and torch.equal(h[keep], h0[keep]) and torch.isfinite(s[keep]).all()
+
+
+@gpu
+def test_no_rows_and_leading_dimensions():
+    announce("gated norm: no rows, three dimensions")
+    import gated_norm_binding as gn
+    e, v = torch.empty(0, 40, device="cuda"), torch.ones(40, device="cuda")
+    y, h = gn.gated_norm(e, e, gate=v)
+    assert y.shape == h.shape == (0, 40)
+    y, q, s = gn.gated_norm_int8(e, e)
+    assert q.shape == (0, 40) and s.shape == (0,)
+    g = gn.gated_norm_backward(e, e, e, e, gate=v, pre_gamma=v)
+    assert g["x"].shape == (0, 40) and not g["gate"].any() and not g["pre_gamma"].any() and g["post_gamma"] is None
+    x, f = values(1, 2, 3, 40).cuda(), values(2, 2, 3, 40).cuda()
+    gate = values(3, 2, 40).cuda()
+    y, h = gn.gated_norm(x, f, gate=gate)
+    y2, h2 = gn.gated_norm(x.view(6, 40), f.view(6, 40), gate=gate)
+    assert y.shape == x.shape and torch.equal(y.view(6, 40), y2) and torch.equal(h.view(6, 40), h2)
+
+
+@gpu
+def test_rows_beyond_two_gib():
+    announce("gated norm: offsets beyond 2^31")
+    import gated_norm_binding as gn
+    rows, wide, cols = 70000, 32800, 48
+    big = torch.empty((rows, wide), dtype=torch.float16, device="cuda")
+    x, src, f = big[:, 32700:32700 + cols], values(9, rows, cols, dtype=torch.float16).cuda(), values(8, rows, cols, dtype=torch.float16).cuda()
+    x.copy_(src)
+    for a, b in zip(gn.gated_norm(x, f), gn.gated_norm(src, f)):
+        assert torch.equal(a, b)
+    for a, b in zip(gn.gated_norm_backward(f, f, x, f).values(), gn.gated_norm_backward(f, f, src, f).values()):
+        assert (a is None and b is None) or torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------- together, as they are used ----
+def block(x, f, p1, w1, b1, w2, b2, p2):
+    """The MLP of a transformer block: the norm in front of it hands over 8-bit rows, the norm behind it takes its output."""
+    import gated_norm_binding as gn
+    import linear_int8_binding as lb
+    y, q, s = gn.gated_norm_int8(x, f, **p1)
+    u = lb.gemm_int8(q, s, w1, bias=b1, act="gelu_tanh", dtype=x.dtype)
+    m = lb.linear_int8(u, w2, bias=b2)
+    y2, h2 = gn.gated_norm(y, m, **p2)
+    return y, q, s, u, m, y2, h2
+
+
+def block_inputs(rows, D, F, t, seed):
+    import linear_int8_binding as lb
+    x, f = values(seed, rows, D, dtype=t).cuda(), values(seed + 1, rows, D, dtype=t).cuda()
+    p1, p2 = (cuda(params(seed + 10 * i, rows, D, t, "layer", "layer", "channel")) for i in (1, 2))
+    w1, w2 = lb.quantize_weight(values(seed + 2, D, F, std=D ** -0.5).cuda()), lb.quantize_weight(values(seed + 3, F, D, std=F ** -0.5).cuda())
+    return x, f, p1, w1, values(seed + 4, F, dtype=t).cuda(), w2, values(seed + 5, D, dtype=t).cuda(), p2
+
+
+def unpack(w):
+    K, N = w.in_features, w.out_features
+    from test_linear_int8 import packed_index
+    return w.packed.cpu()[torch.from_numpy(packed_index(K, N))]
+
+
+@gpu
+@pytest.mark.parametrize("rows,D,F,dtype", [(1, 768, 1000, "f16"), (49, 256, 1024, "bf16"), (300, 130, 500, "f32")])
+def test_block_step_by_step(rows, D, F, dtype):
+    """Every step of the block against 64 bits from what the step before handed over."""
+    announce("block of gated norms and 8-bit layers %d x %d x %d %s" % (rows, D, F, dtype))
+    t = TYPES[dtype]
+    x, f, p1, w1, b1, w2, b2, p2 = block_inputs(rows, D, F, t, 100)
+    y, q, s, u, m, y2, h2 = block(x, f, p1, w1, b1, w2, b2, p2)
+    ry, rh, ey, eh = ref.forward(x, f, p1)
+    ref.check("y", y, ry, ey + ref.half_step(ry, t))
+    assert ((q.double().cpu() * s.double().cpu()[:, None] - rh).abs() <= 0.5 * s.double().cpu()[:, None] * (1 + 2.0 ** -20) + eh).all()
+    r, e = ref.linear(q.cpu(), s.cpu(), unpack(w1), w1.scale.cpu(), b1.cpu(), "gelu_tanh")
+    ref.check("first layer", u, r, e + ref.half_step(r, t))
+    r, e = ref.linear(*ref.quantize(u.cpu()), unpack(w2), w2.scale.cpu(), b2.cpu(), None)
+    ref.check("second layer", m, r, e + ref.half_step(r, t))
+    ry, rh, ey, eh = ref.forward(y.cpu(), m.cpu(), p2)
+    ref.check("y of the next block", y2, ry, ey + ref.half_step(ry, t))
+    ref.check("h of the next block", h2, rh, eh + ref.half_step(rh, t))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 80])
+def test_block_and_gradient_in_a_graph_and_on_another_stream(rows):
+    """Captured once and replayed on new inputs with eager work in between, and on a stream of its own: the eager bits."""
+    announce("block in a graph, rows=%d" % rows)
+    import gated_norm_binding as gn
+    x, f, p1, w1, b1, w2, b2, p2 = block_inputs(rows, 192, 320, torch.float16, 200)
+
+    def everything(x, f):
+        out = block(x, f, p1, w1, b1, w2, b2, p2)
+        g = gn.gated_norm_backward(out[5], out[6], x, f, **p1)
+        return list(out) + [v for v in g.values() if v is not None]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = everything(x, f)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(on_side, everything(x, f)):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = everything(x, f)
+    for i in range(4):
+        nx, nf = values(300 + i, rows, 192, dtype=torch.float16).cuda(), values(400 + i, rows, 192, dtype=torch.float16).cuda()
+        eager = everything(nx, nf)
+        x.copy_(nx)
+        f.copy_(nf)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, eager):
+            assert torch.equal(a, b), "replay %d" % i
+
+
+@gpu
+def test_post_norm_encoder_form():
+    """LN(x + f) of a post-norm encoder: no norm behind the block, no gate, y not kept."""
+    announce("gated norm as LN(x + f)")
+    import gated_norm_binding as gn
+    x, f, g, b = values(1, 64, 768, dtype=torch.float16), values(2, 64, 768, dtype=torch.float16), values(3, 768, dtype=torch.float16), values(4, 768, dtype=torch.float16)
+    y, h = gn.gated_norm(x.cuda(), f.cuda(), post_norm=None, pre_gamma=g.cuda(), pre_beta=b.cuda(), pre_eps=1e-12, want_y=False)
+    p = {"post_norm": None, "pre_gamma": g, "pre_beta": b, "pre_eps": 1e-12}
+    _, rh, _, eh = ref.forward(x, f, p)
+    ref.check("h", h, rh, eh + ref.half_step(rh, torch.float16))
+    r = torch.nn.functional.layer_norm(x.double() + f.double(), (768,), g.double(), b.double(), 1e-12)
+    assert y is None and (rh - r).abs().max() < 1e-10
