@@ -13,6 +13,8 @@
 // results are the columns 16 g + 4 t .. + 3 of one row (g = lane / 16), so over the four operands a lane owns 16 adjacent columns of a row: 32
 // bytes of an fp16 result.
 #include <algorithm>
+#include <atomic>
+#include <cstdlib>
 #include "typed.hpp"
 #include "host_util.hpp"
 
@@ -129,18 +131,31 @@ struct Args {
 
 // NaN stays NaN in all of them.  The tanh GELU in its logistic form v / (1 + exp(-2 u)), u = 0.79788456 (v + 0.044715 v^3): exact
 // in both tails (1 - 1 / (1 + exp 2u) would lose the negative one's digits) and right for infinities.
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act == SOUFFLE_ACT_RELU) return v < 0.f ? 0.f : v;
-  if (act == SOUFFLE_ACT_GELU_TANH) {
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+  if constexpr (ACT == SOUFFLE_ACT_RELU) return v < 0.f ? 0.f : v;
+  if constexpr (ACT == SOUFFLE_ACT_GELU_TANH) {
     constexpr float K1 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, K2 = K1 * 0.044715f;
     return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * __builtin_fmaf(v * v, K2, K1)));
   }
-  if (act == SOUFFLE_ACT_GELU_ERF) return gelu_erf(v);
+  if constexpr (ACT == SOUFFLE_ACT_GELU_ERF) return gelu_erf(v);
   return v;
+}
+template <int ACT>
+struct ActTag {
+  static constexpr int value = ACT;
+};
+// `f(tag)` with the activation as a constant: one branch per epilogue, not one per value.
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+  if (act == SOUFFLE_ACT_NONE) f(ActTag<SOUFFLE_ACT_NONE>());
+  else if (act == SOUFFLE_ACT_RELU) f(ActTag<SOUFFLE_ACT_RELU>());
+  else if (act == SOUFFLE_ACT_GELU_TANH) f(ActTag<SOUFFLE_ACT_GELU_TANH>());
+  else f(ActTag<SOUFFLE_ACT_GELU_ERF>());
 }
 
 // Columns n .. n+3 of row m.
-template <class T>
+template <class T, int ACT>
 __device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s) {
   if (m >= a.M || n >= a.N) return;
   const float rs = a.row_scale[m];
@@ -153,7 +168,7 @@ __device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s) {
   for (int e = 0; e < 4; ++e) {
     const int c = min(n + e, a.N - 1);
     const float v = ((float)s[e] * a.col_scale[c]) * rs + (bias ? (float)bias[c] : 0.f);
-    out[e] = (T)activate(v, a.act);
+    out[e] = (T)activate<ACT>(v);
   }
   if (n + 4 <= a.N) {
     *reinterpret_cast<V4u *>(y) = out;
@@ -214,13 +229,139 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
 #pragma unroll
     for (int j = 0; j < NF; ++j) lds[wave][i * NF + j][lane] = acc[i][j];
   __syncthreads();
-  for (int u = threadIdx.x; u < MF * NF * 64; u += W * 64) {
-    const int tile = u >> 6, l = u & 63;
-    i4 s = lds[0][tile][l];
+  with_activation(a.act, [&](auto act) {
+    for (int u = threadIdx.x; u < MF * NF * 64; u += W * 64) {
+      const int tile = u >> 6, l = u & 63;
+      i4 s = lds[0][tile][l];
 #pragma unroll
-    for (int w = 1; w < W; ++w) s += lds[w][tile][l];
-    finish4<T>(a, m0 + 16 * (tile / NF) + (l & 15), group * 64 + 16 * (l >> 4) + 4 * (t0 + tile % NF), s);
+      for (int w = 1; w < W; ++w) s += lds[w][tile][l];
+      finish4<T, decltype(act)::value>(a, m0 + 16 * (tile / NF) + (l & 15), group * 64 + 16 * (l >> 4) + 4 * (t0 + tile % NF), s);
+    }
+  });
+}
+
+// Columns n .. n+15 of row m, with the scales and the bias of the 16 columns in registers.
+template <class T, int ACT>
+__device__ __forceinline__ void finish16(const Args &a, int m, int n, const i4 (&s)[4], const float (&cs)[16], const float (&bias)[16]) {
+  if (m >= a.M || n >= a.N) return;
+  const float rs = a.row_scale[m];
+  T *y = static_cast<T *>(a.y) + m * a.ldy;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = 8 * half + e;
+      v[e] = activate<ACT>(((float)s[c >> 2][c & 3] * cs[c]) * rs + bias[c]);
+    }
+    store8(y, n + 8 * half, a.N, from_f32<T>(v));
   }
+}
+
+__device__ const int8_t zero_bytes[16] __attribute__((aligned(16))) = {};
+
+// Many rows: a workgroup of WM x WN waves computes 16 MI WM rows x 64 WN columns, 128 of K at a time.  A wave holds MI x 4 accumulator
+// tiles.  The rows go through LDS (every wave of a row of waves needs them) in a ring of three stages filled by
+// direct loads, two steps ahead; the packed weights go straight into registers one step ahead, a wave's 64 columns being 4 KB in a
+// row per 64 of K: through LDS as well they would double its traffic, which at 128 bytes a cycle is
+// what runs out first (a 256 x 256 tile then asks for 64 + 32 + 32 bytes per cycle of matrix instructions).
+//
+// LDS stage [BM rows][8 slots of 16 bytes]: slot p of row r holds bytes 16 (p ^ (r & 7)) .. + 15 of the row's 128, so that the 16
+// rows of an operand read lie in different banks; a direct load of 8 rows x 128 bytes fills 1 KB.
+template <class T, int MI, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
+  constexpr int kWaves = WM * WN, kBM = 16 * MI * WM, kStage = kBM * 128, kLoads = kBM / 8 / kWaves, kWLoads = 8;
+  static_assert(kLoads * kWaves * 8 == kBM, "every wave fills the same number of KB of a stage");
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  // Workgroup b runs on XCD b % 8: each XCD takes a run of tiles, eight rows of tiles deep, so that what its L2 holds is shared.
+  const int row_tiles = (a.M + kBM - 1) / kBM, tiles = row_tiles * a.col_tiles;
+  const int per_xcd = tiles / 8, left = tiles % 8, xcd = blockIdx.x % 8;
+  const int tile = xcd * per_xcd + min(xcd, left) + blockIdx.x / 8;
+  const int band = tile / (8 * a.col_tiles), deep = min(8, row_tiles - 8 * band), in_band = tile - band * 8 * a.col_tiles;
+  const int m0 = (band * 8 + in_band % deep) * kBM, group = in_band / deep * WN + wn, last_group = (a.N + 63) / 64 - 1;
+
+  const unsigned lds0 = lds_address(lds);
+  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16, k_end = a.kblocks * 64;
+  const int8_t *src[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) src[i] = a.q + min(m0 + (wave * kLoads + i) * 8 + (lane >> 3), a.M - 1) * a.ldq;
+  // (behind K's end: zeros, so that steps come in pairs, always with the same loads, and the loop has no branch)
+  auto stage_in = [&](int s, int slot) {
+    const int off = s * 128 + chunk;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_lds16(off < k_end ? src[i] + off : zero_bytes, lds0 + slot * kStage + (wave * kLoads + i) * 1024);
+  };
+  const int8_t *wp = a.packed + (size_t)min(group, last_group) * a.kblocks * 4096 + lane * 16;
+  auto fetch_w = [&](i4 (&w)[2][4], int s) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int8_t *p = wp + (size_t)min(2 * s + h, a.kblocks - 1) * 4096;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[h][j] = ldg16(p + j * 1024);
+    }
+  };
+  i4 acc[MI][4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = i4{0, 0, 0, 0};
+  const int r = lane & 15, g = lane >> 4;
+  const unsigned char *rows = lds + (wm * 16 * MI + r) * 128;
+  auto row16 = [&](int slot, int i, int h) {
+    return __builtin_bit_cast(i4, lds_load16(rows + slot * kStage + i * 2048 + (((h * 4 + g) ^ (r & 7)) * 16)));
+  };
+  // 64 of K: half h of a stage
+  auto multiply = [&](int slot, int h, const i4 (&w)[4], int from, int to) {
+#pragma unroll
+    for (int i = from; i < to; ++i) {
+      const i4 x = row16(slot, i, h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(w[j], x, acc[i][j]);
+    }
+  };
+  // Stage s of the ring with its weights in w; those of s + 1 go to wnext.  A wave's loads are queued in the order
+  // rows of s + 1 | weights of s + 1, rows of s + 2 | ...  The compiler waits for weights at their first use and does not count
+  // the direct loads, so a step's direct loads are queued behind the last first use, where its count, too small by
+  // that many, only asks for loads that are a step old; the explicit wait makes sure of the rows of s + 1.
+  auto step = [&](int s, int slot, i4 (&w)[2][4], i4 (&wnext)[2][4]) {
+    fetch_w(wnext, s + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(slot, 0, w[0], 0, MI);
+    multiply(slot, 1, w[1], 0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    stage_in(s + 2, slot == 0 ? 2 : slot - 1);
+    multiply(slot, 1, w[1], 1, MI);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kWLoads + kLoads) : "memory");
+    __builtin_amdgcn_s_barrier();
+    compiler_fence();
+  };
+  i4 w0[2][4], w1[2][4];
+  stage_in(0, 0);
+  stage_in(1, 1);
+  fetch_w(w0, 0);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWLoads + kLoads) : "memory");
+  __builtin_amdgcn_s_barrier();
+  compiler_fence();
+  for (int s = 0, slot = 0; 2 * s < a.kblocks; s += 2) {
+    step(s, slot, w0, w1);
+    slot = slot == 2 ? 0 : slot + 1;
+    step(s + 1, slot, w1, w0);
+    slot = slot == 2 ? 0 : slot + 1;
+  }
+  wait_vmcnt<0>();      // no direct load is under way when the workgroup gives its LDS back
+  const int n = group * 64 + 16 * g;
+  float cs[16], bias[16];
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    const int at = min(n + c, a.N - 1);
+    cs[c] = a.col_scale[at];
+    bias[c] = a.bias ? (float)static_cast<const T *>(a.bias)[at] : 0.f;
+  }
+  with_activation(a.act, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) finish16<T, decltype(act)::value>(a, m0 + (wm * MI + i) * 16 + r, n, acc[i], cs, bias);
+  });
 }
 
 // ------------------------------------------------------------------------------------------- host side ----
@@ -273,11 +414,39 @@ static int launch_split(Args a, hipStream_t st) {
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
+template <class T, int MI, int WM, int WN>
+static int launch_tile(Args a, hipStream_t st) {
+  constexpr int kBM = 16 * MI * WM, kLds = 3 * kBM * 128;
+  static std::atomic<unsigned> done{0};      // devices whose copy of the kernel may use that much LDS
+  int dev = 0;
+  SOUFFLE_HIP_TRY(hipGetDevice(&dev));
+  if (!(done.load() >> dev & 1)) {
+    SOUFFLE_HIP_TRY(hipFuncSetAttribute((const void *)k_gemm_tile<T, MI, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+    done.fetch_or(1u << dev);
+  }
+  a.col_tiles = (a.N + 64 * WN - 1) / (64 * WN);
+  const long long grid = (long long)a.col_tiles * ((a.M + kBM - 1) / kBM);
+  if (grid > 0x7fffffff) return fail(SOUFFLE_ERR_SHAPE, "M = %d rows of N = %d are more tiles than one launch holds", a.M, a.N);
+  hipLaunchKernelGGL((k_gemm_tile<T, MI, WM, WN>), dim3((unsigned)grid), dim3(WM * WN * 64), kLds, st, a);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
 template <class T>
 static int gemm(const Args &a, hipStream_t st) {
   if (a.M <= 16) return launch_split<T, 1, 1, 8, 4>(a, st);
   if (a.M <= 32) return launch_split<T, 2, 1, 8, 4>(a, st);
-  return launch_split<T, 4, 4, 4, 1>(a, st);
+  const int force = getenv("SOUFFLE_TILE") ? atoi(getenv("SOUFFLE_TILE")) : -1;
+  if (force == 0) return launch_split<T, 4, 4, 4, 1>(a, st);
+  if (force == 1) return launch_tile<T, 4, 1, 2>(a, st);
+  if (force == 2) return launch_tile<T, 4, 2, 2>(a, st);
+  if (force == 3) return launch_tile<T, 4, 2, 4>(a, st);
+  if (force == 4) return launch_tile<T, 8, 2, 4>(a, st);
+  if (force == 5) return launch_tile<T, 8, 1, 4>(a, st);
+  if (force == 6) return launch_tile<T, 2, 2, 2>(a, st);
+  if (force == 7) return launch_split<T, 2, 4, 8, 1>(a, st);
+  if (force == 8) return launch_split<T, 4, 1, 8, 2>(a, st);
+  if (a.M <= 64) return launch_split<T, 4, 4, 4, 1>(a, st);
+  return launch_tile<T, 8, 2, 4>(a, st);
 }
 static int gemm(const Args &a, int dtype, hipStream_t st) {
   if (dtype == SOUFFLE_F16) return gemm<half_t>(a, st);
