@@ -27,6 +27,14 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 // of A (of B), and rows 4 (l / 16) .. + 3 of column l % 16 of D.
 __device__ __forceinline__ i4 mfma_i8(i4 a, i4 b, i4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
+// The 4-byte form of load_lds16: lane L's word lands at lds_addr + 4 L.
+__device__ __forceinline__ void load_lds4(const void *src, unsigned lds_addr) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(src) : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
 __device__ __forceinline__ i4 ldg16(const int8_t *p) { return *(const __attribute__((address_space(1))) i4 *)p; }
 
 // ---------------------------------------------------------------------------------------- quantisation ----
@@ -184,39 +192,41 @@ __device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s) {
 // the loop has no barrier), and the W partial sums meet in LDS at the end.
 template <class T, int MF, int NF, int W, int U>
 __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
-  static_assert(NF == 1 || NF == 4, "one operand, or the four of 64 columns");
+  static_assert(4 % NF == 0, "operands of the four that 64 columns have");
   __shared__ i4 lds[W][MF * NF][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = blockIdx.x % a.col_tiles, group = NF == 4 ? col : col >> 2, t0 = NF == 4 ? 0 : col & 3, m0 = blockIdx.x / a.col_tiles * 16 * MF;
+  constexpr int kParts = 4 / NF;
+  const int col = blockIdx.x % a.col_tiles, group = col / kParts, t0 = col % kParts * NF, m0 = blockIdx.x / a.col_tiles * 16 * MF;
   i4 acc[MF][NF] = {};
   const int8_t *wp = a.packed + ((size_t)group * a.kblocks * 4 + t0) * 1024 + lane * 16;
   const int8_t *xp[MF];
 #pragma unroll
   for (int i = 0; i < MF; ++i) xp[i] = a.q + min(m0 + 16 * i + (lane & 15), a.M - 1) * a.ldq + 16 * (lane >> 4);
-  // U of the wave's steps at a time, the next U loaded while the present ones are multiplied.  A step behind K's end reads the
-  // last one's operands again, with the weights replaced by zeros.
+  // The wave's part of K, U steps at a time, the next U loaded while the present ones are multiplied.  (A step behind the
+  // part's end reads its last operands again, with the weights replaced by zeros.)
+  const int part = (a.kblocks + W - 1) / W, k_first = wave * part, k_end = min(k_first + part, a.kblocks);
   i4 wv[U][NF], xv[U][MF];
   auto fetch = [&](int kb) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = min(kb + u * W, a.kblocks - 1);
+      const int k = min(kb + u, k_end - 1);
 #pragma unroll
       for (int j = 0; j < NF; ++j) wv[u][j] = ldg16(wp + (size_t)k * 4096 + j * 1024);
 #pragma unroll
       for (int i = 0; i < MF; ++i) xv[u][i] = ldg16(xp[i] + k * 64);
     }
   };
-  fetch(wave);
-  for (int kb = wave; kb < a.kblocks; kb += U * W) {
+  if (k_first < k_end) fetch(k_first);
+  for (int kb = k_first; kb < k_end; kb += U) {
     i4 wn[U][NF], xn[U][MF];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) wn[u][j] = kb + u * W < a.kblocks ? wv[u][j] : i4{0, 0, 0, 0};
+      for (int j = 0; j < NF; ++j) wn[u][j] = kb + u < k_end ? wv[u][j] : i4{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < MF; ++i) xn[u][i] = xv[u][i];
     }
-    if (kb + U * W < a.kblocks) fetch(kb + U * W);
+    if (kb + U < k_end) fetch(kb + U);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -240,21 +250,66 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
   });
 }
 
-// Columns n .. n+15 of row m, with the scales and the bias of the 16 columns in registers.
+// Rows of 16 lanes: the odd ones of a change places with the even ones of b (permlane16), the upper two of a with the lower two of b (permlane32).
+template <class V>
+__device__ __forceinline__ void swap16(V &a, V &b) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const auto p = __builtin_amdgcn_permlane16_swap(a[e], b[e], false, false);
+    a[e] = p[0];
+    b[e] = p[1];
+  }
+}
+template <class V>
+__device__ __forceinline__ void swap32(V &a, V &b) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const auto p = __builtin_amdgcn_permlane32_swap(a[e], b[e], false, false);
+    a[e] = p[0];
+    b[e] = p[1];
+  }
+}
+// The 64 columns from n0 of row m, 16 of them (from 16 g, g = lane / 16) in this lane, with their scales and bias in registers.  The
+// 16-byte pieces change places between the four lanes of a row, so that these store 64 bytes in a row each time.
 template <class T, int ACT>
-__device__ __forceinline__ void finish16(const Args &a, int m, int n, const i4 (&s)[4], const float (&cs)[16], const float (&bias)[16]) {
-  if (m >= a.M || n >= a.N) return;
-  const float rs = a.row_scale[m];
+__device__ __forceinline__ void finish16(const Args &a, int m, int n0, const i4 (&s)[4], float rs, const float (&cs)[16], const float (&bias)[16]) {
+  const int g = (threadIdx.x & 63) >> 4;
+  constexpr int kPer = 16 / sizeof(T), kPieces = 16 / kPer;      // elements of a piece; pieces of a lane
+  u4 piece[kPieces];
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    typedef T V __attribute__((ext_vector_type(kPer)));
+    V v;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int c = kPer * k + e;
+      v[e] = (T)activate<ACT>(((float)s[c >> 2][c & 3] * cs[c]) * rs + bias[c]);
+    }
+    piece[k] = __builtin_bit_cast(u4, v);
+  }
+  swap16(piece[0], piece[1]);
+  if constexpr (kPieces == 2) {
+    swap32(piece[0], piece[1]);
+  } else {
+    swap16(piece[2], piece[3]);
+    swap32(piece[0], piece[2]);
+    swap32(piece[1], piece[3]);
+  }
+  if (m >= a.M) return;
   T *y = static_cast<T *>(a.y) + m * a.ldy;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float v[8];
+  for (int k = 0; k < kPieces; ++k) {
+    const int n = n0 + (4 * k + g) * kPer;
+    typedef T V __attribute__((ext_vector_type(kPer)));
+    typedef T Vu __attribute__((ext_vector_type(kPer), aligned(sizeof(T))));
+    const V v = __builtin_bit_cast(V, piece[k]);
+    if (n + kPer <= a.N) {
+      *(__attribute__((address_space(1))) Vu *)(y + n) = v;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = 8 * half + e;
-      v[e] = activate<ACT>(((float)s[c >> 2][c & 3] * cs[c]) * rs + bias[c]);
+      for (int e = 0; e < kPer; ++e)
+        if (n + e < a.N) y[n + e] = v[e];
     }
-    store8(y, n + 8 * half, a.N, from_f32<T>(v));
   }
 }
 
@@ -266,8 +321,8 @@ __device__ const int8_t zero_bytes[16] __attribute__((aligned(16))) = {};
 // row per 64 of K: through LDS as well they would double its traffic, which at 128 bytes a cycle is
 // what runs out first (a 256 x 256 tile then asks for 64 + 32 + 32 bytes per cycle of matrix instructions).
 //
-// LDS stage [BM rows][8 slots of 16 bytes]: slot p of row r holds bytes 16 (p ^ (r & 7)) .. + 15 of the row's 128, so that the 16
-// rows of an operand read lie in different banks; a direct load of 8 rows x 128 bytes fills 1 KB.
+// LDS stage [BM rows][8 slots of 16 bytes]: slot p of row r holds bytes 16 (p ^ (r / 2 % 8)) .. + 15 of the row's 128, so that the 16
+// rows of an operand read lie in different banks (64 banks are two rows); a direct load of 8 rows x 128 bytes fills 1 KB.
 template <class T, int MI, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
   constexpr int kWaves = WM * WN, kBM = 16 * MI * WM, kStage = kBM * 128, kLoads = kBM / 8 / kWaves, kWLoads = 8;
@@ -282,15 +337,22 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
   const int m0 = (band * 8 + in_band % deep) * kBM, group = in_band / deep * WN + wn, last_group = (a.N + 63) / 64 - 1;
 
   const unsigned lds0 = lds_address(lds);
-  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16, k_end = a.kblocks * 64;
+  const int k_end = a.kblocks * 64;
   const int8_t *src[kLoads];
+  int chunk[kLoads];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) src[i] = a.q + min(m0 + (wave * kLoads + i) * 8 + (lane >> 3), a.M - 1) * a.ldq;
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = (wave * kLoads + i) * 8 + (lane >> 3);
+    src[i] = a.q + min(m0 + row, a.M - 1) * a.ldq;
+    chunk[i] = ((lane & 7) ^ (row >> 1 & 7)) * 16;
+  }
   // (behind K's end: zeros, so that steps come in pairs, always with the same loads, and the loop has no branch)
   auto stage_in = [&](int s, int slot) {
-    const int off = s * 128 + chunk;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_lds16(off < k_end ? src[i] + off : zero_bytes, lds0 + slot * kStage + (wave * kLoads + i) * 1024);
+    for (int i = 0; i < kLoads; ++i) {
+      const int off = s * 128 + chunk[i];
+      load_lds16(off < k_end ? src[i] + off : zero_bytes, lds0 + slot * kStage + (wave * kLoads + i) * 1024);
+    }
   };
   const int8_t *wp = a.packed + (size_t)min(group, last_group) * a.kblocks * 4096 + lane * 16;
   auto fetch_w = [&](i4 (&w)[2][4], int s) {
@@ -309,33 +371,42 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
   const int r = lane & 15, g = lane >> 4;
   const unsigned char *rows = lds + (wm * 16 * MI + r) * 128;
   auto row16 = [&](int slot, int i, int h) {
-    return __builtin_bit_cast(i4, lds_load16(rows + slot * kStage + i * 2048 + (((h * 4 + g) ^ (r & 7)) * 16)));
+    return __builtin_bit_cast(i4, lds_load16(rows + slot * kStage + i * 2048 + (((h * 4 + g) ^ (r >> 1 & 7)) * 16)));
   };
-  // 64 of K: half h of a stage
-  auto multiply = [&](int slot, int h, const i4 (&w)[4], int from, int to) {
-#pragma unroll
-    for (int i = from; i < to; ++i) {
-      const i4 x = row16(slot, i, h);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(w[j], x, acc[i][j]);
-    }
-  };
-  // Stage s of the ring with its weights in w; those of s + 1 go to wnext.  A wave's loads are queued in the order
-  // rows of s + 1 | weights of s + 1, rows of s + 2 | ...  The compiler waits for weights at their first use and does not count
-  // the direct loads, so a step's direct loads are queued behind the last first use, where its count, too small by
-  // that many, only asks for loads that are a step old; the explicit wait makes sure of the rows of s + 1.
+  // Stage s of the ring with its weights in w; those of s + 1 go to wnext.  The 2 MI operands of rows are read two ahead of their use, across
+  // the step's end, so the one barrier of a step stands in its middle: it says that the rows of s + 1 are there and that nobody reads
+  // those of s - 1 any more.  A wave's loads are queued in the order weights of s + 1, rows of s + 2 | ...  The
+  // compiler waits for weights at their first use and does not count the direct loads, so these are queued behind
+  // the step's last first use: its count, too small by that many, then only asks for loads that are a step old.
+  i4 x0, x1;
   auto step = [&](int s, int slot, i4 (&w)[2][4], i4 (&wnext)[2][4]) {
+    const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
     fetch_w(wnext, s + 1);
     __builtin_amdgcn_sched_barrier(0);
-    multiply(slot, 0, w[0], 0, MI);
-    multiply(slot, 1, w[1], 0, 1);
-    __builtin_amdgcn_sched_barrier(0);
-    stage_in(s + 2, slot == 0 ? 2 : slot - 1);
-    multiply(slot, 1, w[1], 1, MI);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kWLoads + kLoads) : "memory");
-    __builtin_amdgcn_s_barrier();
-    compiler_fence();
+#pragma unroll
+    for (int u = 0; u < 2 * MI; ++u) {
+      const i4 x2 = u + 2 < 2 * MI ? row16(slot, (u + 2) % MI, (u + 2) / MI) : row16(slot1, u + 2 - 2 * MI, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[u % MI][j] = mfma_i8(w[u / MI][j], x0, acc[u % MI][j]);
+      x0 = x1;
+      x1 = x2;
+      if (u == MI - 1) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWLoads) : "memory");
+        __builtin_amdgcn_s_barrier();
+        compiler_fence();
+      }
+      __builtin_amdgcn_sched_barrier(0);      // (otherwise the reads sink to their uses)
+      if (u == MI) stage_in(s + 2, slot2);
+    }
   };
+  // The scales of the tile's rows and columns wait for the epilogue in LDS, behind the stages.
+  float *row_scale = reinterpret_cast<float *>(lds + 3 * kStage), *col_scale = row_scale + kBM;
+#pragma unroll
+  for (int i = 0; i < (kBM / 64 + WN + kWaves - 1) / kWaves; ++i) {
+    const int part = wave + i * kWaves, c = (in_band / deep * WN + part - kBM / 64) * 64 + lane;
+    const float *from = part < kBM / 64 ? a.row_scale + min(m0 + part * 64 + lane, a.M - 1) : a.col_scale + min(c, a.N - 1);
+    if (part < kBM / 64 + WN) load_lds4(from, lds0 + 3 * kStage + part * 256);
+  }
   i4 w0[2][4], w1[2][4];
   stage_in(0, 0);
   stage_in(1, 1);
@@ -343,6 +414,8 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWLoads + kLoads) : "memory");
   __builtin_amdgcn_s_barrier();
   compiler_fence();
+  x0 = row16(0, 0, 0);
+  x1 = row16(0, 1, 0);
   for (int s = 0, slot = 0; 2 * s < a.kblocks; s += 2) {
     step(s, slot, w0, w1);
     slot = slot == 2 ? 0 : slot + 1;
@@ -354,13 +427,31 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
   float cs[16], bias[16];
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
-    const int at = min(n + c, a.N - 1);
-    cs[c] = a.col_scale[at];
-    bias[c] = a.bias ? (float)static_cast<const T *>(a.bias)[at] : 0.f;
+    cs[c] = col_scale[wn * 64 + 16 * g + c];
+    bias[c] = 0.f;
   }
-  with_activation(a.act, [&](auto act) {
+  if (a.bias) {
+    float b[2][8];
 #pragma unroll
-    for (int i = 0; i < MI; ++i) finish16<T, decltype(act)::value>(a, m0 + (wm * MI + i) * 16 + r, n, acc[i], cs, bias);
+    for (int half = 0; half < 2; ++half) {
+      to_f32(b[half], load8(static_cast<const T *>(a.bias), n + 8 * half, a.N));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bias[8 * half + e] = b[half][e];
+    }
+  }
+  // One row tile at a time through one copy of the code: unrolled, the epilogue is 64 lines of instructions that every launch
+  // fetches once and runs once.
+  with_activation(a.act, [&](auto act) {
+#pragma unroll 1
+    for (int i = 0; i < MI; ++i) {
+      i4 v[4];
+#pragma unroll
+      for (int k = 0; k < MI; ++k)
+        if (i == k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = acc[k][j];
+      finish16<T, decltype(act)::value>(a, m0 + (wm * MI + i) * 16 + r, group * 64, v, row_scale[(wm * MI + i) * 16 + r], cs, bias);
+    }
   });
 }
 
@@ -416,7 +507,7 @@ static int launch_split(Args a, hipStream_t st) {
 }
 template <class T, int MI, int WM, int WN>
 static int launch_tile(Args a, hipStream_t st) {
-  constexpr int kBM = 16 * MI * WM, kLds = 3 * kBM * 128;
+  constexpr int kBM = 16 * MI * WM, kLds = 3 * kBM * 128 + (kBM + 64 * WN) * 4;
   static std::atomic<unsigned> done{0};      // devices whose copy of the kernel may use that much LDS
   int dev = 0;
   SOUFFLE_HIP_TRY(hipGetDevice(&dev));
@@ -433,18 +524,28 @@ static int launch_tile(Args a, hipStream_t st) {
 }
 template <class T>
 static int gemm(const Args &a, hipStream_t st) {
-  if (a.M <= 16) return launch_split<T, 1, 1, 8, 4>(a, st);
-  if (a.M <= 32) return launch_split<T, 2, 1, 8, 4>(a, st);
   const int force = getenv("SOUFFLE_TILE") ? atoi(getenv("SOUFFLE_TILE")) : -1;
-  if (force == 0) return launch_split<T, 4, 4, 4, 1>(a, st);
-  if (force == 1) return launch_tile<T, 4, 1, 2>(a, st);
-  if (force == 2) return launch_tile<T, 4, 2, 2>(a, st);
-  if (force == 3) return launch_tile<T, 4, 2, 4>(a, st);
-  if (force == 4) return launch_tile<T, 8, 2, 4>(a, st);
-  if (force == 5) return launch_tile<T, 8, 1, 4>(a, st);
-  if (force == 6) return launch_tile<T, 2, 2, 2>(a, st);
-  if (force == 7) return launch_split<T, 2, 4, 8, 1>(a, st);
-  if (force == 8) return launch_split<T, 4, 1, 8, 2>(a, st);
+  if (force == 0) return launch_split<T, 1, 1, 8, 4>(a, st);
+  if (force == 1) return launch_split<T, 1, 1, 16, 4>(a, st);
+  if (force == 2) return launch_split<T, 1, 2, 8, 4>(a, st);
+  if (force == 3) return launch_split<T, 1, 2, 16, 2>(a, st);
+  if (force == 4) return launch_split<T, 1, 4, 8, 2>(a, st);
+  if (force == 5) return launch_split<T, 1, 4, 16, 2>(a, st);
+  if (force == 6) return launch_split<T, 2, 1, 8, 4>(a, st);
+  if (force == 7) return launch_split<T, 2, 1, 16, 2>(a, st);
+  if (force == 8) return launch_split<T, 2, 2, 8, 2>(a, st);
+  if (force == 9) return launch_split<T, 2, 2, 16, 2>(a, st);
+  if (force == 10) return launch_split<T, 2, 4, 8, 2>(a, st);
+  if (force == 11) return launch_split<T, 2, 4, 8, 1>(a, st);
+  if (force == 12) return launch_split<T, 2, 4, 16, 1>(a, st);
+  if (force == 13) return launch_split<T, 4, 4, 8, 1>(a, st);
+  if (force == 14) return launch_split<T, 4, 2, 8, 1>(a, st);
+  if (force == 15) return launch_split<T, 4, 2, 16, 1>(a, st);
+  if (force == 16) return launch_tile<T, 2, 2, 2>(a, st);
+  if (force == 17) return launch_tile<T, 4, 1, 2>(a, st);
+  if (force == 18) return launch_tile<T, 4, 2, 2>(a, st);
+  if (force == 19) return launch_tile<T, 4, 2, 4>(a, st);
+  if (force == 20) return launch_tile<T, 8, 2, 4>(a, st);
   if (a.M <= 64) return launch_split<T, 4, 4, 4, 1>(a, st);
   return launch_tile<T, 8, 2, 4>(a, st);
 }
