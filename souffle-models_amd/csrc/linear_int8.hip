@@ -124,9 +124,11 @@ __global__ void __launch_bounds__(256) k_pack_weight(const W *w, long long ldw, 
 
 // -------------------------------------------------------------------------------------------- products ----
 struct Args {
-  const int8_t *q;
+  const int8_t *q;               // rows and their scales, or
   long long ldq;
   const float *row_scale;
+  const void *x;                 // activations that the kernel quantises itself
+  long long ldx;
   const int8_t *packed;
   const float *col_scale;
   const void *bias;              // of the output's type, nullable
@@ -135,6 +137,7 @@ struct Args {
   int M, N, K, act;
   int kblocks;                   // K / 64, rounded up
   int col_tiles;                 // workgroups along N
+  int num_cus;
 };
 
 // NaN stays NaN in all of them.  The tanh GELU in its logistic form v / (1 + exp(-2 u)), u = 0.79788456 (v + 0.044715 v^3): exact
@@ -164,9 +167,7 @@ __device__ __forceinline__ void with_activation(int act, F f) {
 
 // Columns n .. n+3 of row m.
 template <class T, int ACT>
-__device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s) {
-  if (m >= a.M || n >= a.N) return;
-  const float rs = a.row_scale[m];
+__device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s, float rs) {
   T *y = static_cast<T *>(a.y) + m * a.ldy + n;
   const T *bias = static_cast<const T *>(a.bias);
   typedef T V4 __attribute__((ext_vector_type(4)));
@@ -187,23 +188,32 @@ __device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s) {
   }
 }
 
-// Few rows: a workgroup of W waves computes 16 MF rows x 16 NF columns, its waves take turns at K in steps of 64 with both
-// operands straight from memory into registers (nothing is shared between waves, so nothing goes through LDS and
-// the loop has no barrier), and the W partial sums meet in LDS at the end.
-template <class T, int MF, int NF, int W, int U>
+// Few rows: a workgroup of W waves computes 16 MF rows x 16 NF columns, each wave a part of K with both operands straight from
+// memory into registers (nothing is shared between waves, so nothing goes through LDS and the loop has no
+// barrier), and the W partial sums meet in LDS at the end.  A wave's part is contiguous: two steps share the 128-byte
+// lines of the rows.
+//
+// ROWS: the rows come as activations, and every workgroup quantises all of them into LDS itself while its first weights
+// are under way: for a few rows that costs less than a launch of its own in front of this one.
+template <class T, int MF, int NF, int W, int U, bool ROWS>
 __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
   static_assert(4 % NF == 0, "operands of the four that 64 columns have");
-  __shared__ i4 lds[W][MF * NF][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  static_assert(!ROWS || MF == 1, "rows of one operand");
   constexpr int kParts = 4 / NF;
+  __shared__ i4 lds[W][MF * NF][64];
+  __shared__ float lds_scale[16];
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds_rows[];      // ROWS: [M][64 kblocks + 16]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = blockIdx.x % a.col_tiles, group = col / kParts, t0 = col % kParts * NF, m0 = blockIdx.x / a.col_tiles * 16 * MF;
+  const int pitch = a.kblocks * 64 + 16;
   i4 acc[MF][NF] = {};
   const int8_t *wp = a.packed + ((size_t)group * a.kblocks * 4 + t0) * 1024 + lane * 16;
   const int8_t *xp[MF];
+  const unsigned char *xrow = lds_rows + min(lane & 15, a.M - 1) * pitch + 16 * (lane >> 4);
 #pragma unroll
   for (int i = 0; i < MF; ++i) xp[i] = a.q + min(m0 + 16 * i + (lane & 15), a.M - 1) * a.ldq + 16 * (lane >> 4);
-  // The wave's part of K, U steps at a time, the next U loaded while the present ones are multiplied.  (A step behind the
-  // part's end reads its last operands again, with the weights replaced by zeros.)
+  // U steps at a time, the next U loaded while the present ones are multiplied.  (A step behind the part's end reads its
+  // last operands again, with the weights replaced by zeros.)
   const int part = (a.kblocks + W - 1) / W, k_first = wave * part, k_end = min(k_first + part, a.kblocks);
   i4 wv[U][NF], xv[U][MF];
   auto fetch = [&](int kb) {
@@ -212,11 +222,43 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
       const int k = min(kb + u, k_end - 1);
 #pragma unroll
       for (int j = 0; j < NF; ++j) wv[u][j] = ldg16(wp + (size_t)k * 4096 + j * 1024);
+      if constexpr (!ROWS)
 #pragma unroll
-      for (int i = 0; i < MF; ++i) xv[u][i] = ldg16(xp[i] + k * 64);
+        for (int i = 0; i < MF; ++i) xv[u][i] = ldg16(xp[i] + k * 64);
     }
   };
   if (k_first < k_end) fetch(k_first);
+  if constexpr (ROWS) {
+    // as many waves per row as there are for M rows at a time
+    __shared__ unsigned lds_max[2][W];
+    const int per_row = a.M == 1 ? W : a.M == 2 ? W / 2 : a.M <= 4 ? W / 4 : W / 8, slots = W / per_row;
+    const int c0 = (wave % per_row * 64 + lane) * 8, stride = per_row * 512;
+    for (int base = 0, turn = 0; base < a.M; base += slots, turn ^= 1) {
+      const int row = base + wave / per_row;
+      const T *x = static_cast<const T *>(a.x) + min(row, a.M - 1) * a.ldx;
+      typename Vec8<T>::type first = load8(x, c0, a.K);
+      float f[8];
+      unsigned m = 0u;
+      for (int c = c0; c < a.K; c += stride) {
+        to_f32(f, c == c0 ? first : load8(x, c, a.K));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
+      }
+      m = wave_umax_dpp(m);
+      if (lane == 0) lds_max[turn][wave] = m;
+      __syncthreads();
+      for (int w = 0; w < per_row; ++w) m = max(m, lds_max[turn][wave / per_row * per_row + w]);
+      const RowScale rs = row_scale(m);
+      if (row < a.M) {
+        for (int c = c0; c < a.K; c += stride) {
+          to_f32(f, c == c0 ? first : load8(x, c, a.K));
+          *reinterpret_cast<u2 *>(lds_rows + row * pitch + c) = quantize8(f, rs);
+        }
+        if (lane == 0) lds_scale[row] = rs.scale;
+      }
+    }
+    __syncthreads();
+  }
   for (int kb = k_first; kb < k_end; kb += U) {
     i4 wn[U][NF], xn[U][MF];
 #pragma unroll
@@ -224,7 +266,10 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
 #pragma unroll
       for (int j = 0; j < NF; ++j) wn[u][j] = kb + u < k_end ? wv[u][j] : i4{0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < MF; ++i) xn[u][i] = xv[u][i];
+      for (int i = 0; i < MF; ++i) {
+        if constexpr (ROWS) xn[u][i] = __builtin_bit_cast(i4, lds_load16(xrow + min(kb + u, k_end - 1) * 64));
+        else xn[u][i] = xv[u][i];
+      }
     }
     if (kb + U < k_end) fetch(kb + U);
 #pragma unroll
@@ -241,11 +286,11 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
   __syncthreads();
   with_activation(a.act, [&](auto act) {
     for (int u = threadIdx.x; u < MF * NF * 64; u += W * 64) {
-      const int tile = u >> 6, l = u & 63;
+      const int tile = u >> 6, l = u & 63, m = m0 + 16 * (tile / NF) + (l & 15), n = group * 64 + 16 * (l >> 4) + 4 * (t0 + tile % NF);
       i4 s = lds[0][tile][l];
 #pragma unroll
       for (int w = 1; w < W; ++w) s += lds[w][tile][l];
-      finish4<T, decltype(act)::value>(a, m0 + 16 * (tile / NF) + (l & 15), group * 64 + 16 * (l >> 4) + 4 * (t0 + tile % NF), s);
+      if (m < a.M && n < a.N) finish4<T, decltype(act)::value>(a, m, n, s, ROWS ? lds_scale[m] : a.row_scale[m]);
     }
   });
 }
@@ -496,29 +541,47 @@ static int quantize_rows(const void *x, int dtype, long long ldx, int8_t *q, lon
   return quantize_rows<float>(x, ldx, q, ldq, scale, M, K, st);
 }
 
+// One workgroup per tile.  (Tiles narrower than 64 columns interleave: there are 64 / cols of them for any part of 64.)
+static int grid_of(const Args &a, int rows, int cols, unsigned *grid, int *col_tiles) {
+  *col_tiles = cols < 64 ? (a.N + 63) / 64 * (64 / cols) : (a.N + cols - 1) / cols;
+  const long long n = (long long)*col_tiles * ((a.M + rows - 1) / rows);
+  if (n > 0x7fffffff) return fail(SOUFFLE_ERR_SHAPE, "M = %d rows of N = %d are more tiles than one launch holds", a.M, a.N);
+  *grid = (unsigned)n;
+  return SOUFFLE_OK;
+}
+// The kernel may use `bytes` of LDS on the current device (set once per device and kernel).
+static int allow_lds(const void *kernel, int bytes, std::atomic<unsigned> &done) {
+  int dev = 0;
+  SOUFFLE_HIP_TRY(hipGetDevice(&dev));
+  if (done.load() >> dev & 1) return SOUFFLE_OK;
+  SOUFFLE_HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(1u << dev);
+  return SOUFFLE_OK;
+}
 template <class T, int MF, int NF, int W, int U>
 static int launch_split(Args a, hipStream_t st) {
-  a.col_tiles = (a.N + 63) / 64 * (4 / NF);
-  const long long grid = (long long)a.col_tiles * ((a.M + 16 * MF - 1) / (16 * MF));
-  if (grid > 0x7fffffff) return fail(SOUFFLE_ERR_SHAPE, "M = %d rows of N = %d are more tiles than one launch holds", a.M, a.N);
-  hipLaunchKernelGGL((k_gemm_split<T, MF, NF, W, U>), dim3((unsigned)grid), dim3(W * 64), 0, st, a);
+  unsigned grid;
+  if (int rc = grid_of(a, 16 * MF, 16 * NF, &grid, &a.col_tiles)) return rc;
+  hipLaunchKernelGGL((k_gemm_split<T, MF, NF, W, U, false>), dim3(grid), dim3(W * 64), 0, st, a);
+  SOUFFLE_HIP_TRY(hipGetLastError());
+  return SOUFFLE_OK;
+}
+template <class T, int NF, int U>
+static int launch_rows(Args a, hipStream_t st) {
+  unsigned grid;
+  if (int rc = grid_of(a, 16, 16 * NF, &grid, &a.col_tiles)) return rc;
+  hipLaunchKernelGGL((k_gemm_split<T, 1, NF, 8, U, true>), dim3(grid), dim3(512), a.M * (a.kblocks * 64 + 16), st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
 template <class T, int MI, int WM, int WN>
 static int launch_tile(Args a, hipStream_t st) {
   constexpr int kBM = 16 * MI * WM, kLds = 3 * kBM * 128 + (kBM + 64 * WN) * 4;
-  static std::atomic<unsigned> done{0};      // devices whose copy of the kernel may use that much LDS
-  int dev = 0;
-  SOUFFLE_HIP_TRY(hipGetDevice(&dev));
-  if (!(done.load() >> dev & 1)) {
-    SOUFFLE_HIP_TRY(hipFuncSetAttribute((const void *)k_gemm_tile<T, MI, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-    done.fetch_or(1u << dev);
-  }
-  a.col_tiles = (a.N + 64 * WN - 1) / (64 * WN);
-  const long long grid = (long long)a.col_tiles * ((a.M + kBM - 1) / kBM);
-  if (grid > 0x7fffffff) return fail(SOUFFLE_ERR_SHAPE, "M = %d rows of N = %d are more tiles than one launch holds", a.M, a.N);
-  hipLaunchKernelGGL((k_gemm_tile<T, MI, WM, WN>), dim3((unsigned)grid), dim3(WM * WN * 64), kLds, st, a);
+  static std::atomic<unsigned> done{0};
+  if (int rc = allow_lds((const void *)k_gemm_tile<T, MI, WM, WN>, kLds, done)) return rc;
+  unsigned grid;
+  if (int rc = grid_of(a, kBM, 64 * WN, &grid, &a.col_tiles)) return rc;
+  hipLaunchKernelGGL((k_gemm_tile<T, MI, WM, WN>), dim3(grid), dim3(WM * WN * 64), kLds, st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
@@ -526,33 +589,39 @@ template <class T>
 static int gemm(const Args &a, hipStream_t st) {
   const int force = getenv("SOUFFLE_TILE") ? atoi(getenv("SOUFFLE_TILE")) : -1;
   if (force == 0) return launch_split<T, 1, 1, 8, 4>(a, st);
-  if (force == 1) return launch_split<T, 1, 1, 16, 4>(a, st);
-  if (force == 2) return launch_split<T, 1, 2, 8, 4>(a, st);
-  if (force == 3) return launch_split<T, 1, 2, 16, 2>(a, st);
-  if (force == 4) return launch_split<T, 1, 4, 8, 2>(a, st);
-  if (force == 5) return launch_split<T, 1, 4, 16, 2>(a, st);
-  if (force == 6) return launch_split<T, 2, 1, 8, 4>(a, st);
-  if (force == 7) return launch_split<T, 2, 1, 16, 2>(a, st);
-  if (force == 8) return launch_split<T, 2, 2, 8, 2>(a, st);
-  if (force == 9) return launch_split<T, 2, 2, 16, 2>(a, st);
-  if (force == 10) return launch_split<T, 2, 4, 8, 2>(a, st);
-  if (force == 11) return launch_split<T, 2, 4, 8, 1>(a, st);
-  if (force == 12) return launch_split<T, 2, 4, 16, 1>(a, st);
-  if (force == 13) return launch_split<T, 4, 4, 8, 1>(a, st);
-  if (force == 14) return launch_split<T, 4, 2, 8, 1>(a, st);
-  if (force == 15) return launch_split<T, 4, 2, 16, 1>(a, st);
-  if (force == 16) return launch_tile<T, 2, 2, 2>(a, st);
-  if (force == 17) return launch_tile<T, 4, 1, 2>(a, st);
-  if (force == 18) return launch_tile<T, 4, 2, 2>(a, st);
-  if (force == 19) return launch_tile<T, 4, 2, 4>(a, st);
-  if (force == 20) return launch_tile<T, 8, 2, 4>(a, st);
-  if (a.M <= 64) return launch_split<T, 4, 4, 4, 1>(a, st);
-  return launch_tile<T, 8, 2, 4>(a, st);
+  if (force == 1) return launch_split<T, 1, 4, 8, 2>(a, st);
+  if (force == 2) return launch_split<T, 2, 2, 8, 2>(a, st);
+  if (force == 3) return launch_split<T, 2, 4, 8, 1>(a, st);
+  if (force == 4) return launch_tile<T, 2, 2, 2>(a, st);
+  if (force == 5) return launch_tile<T, 4, 1, 2>(a, st);
+  if (force == 6) return launch_tile<T, 4, 2, 2>(a, st);
+  if (force == 7) return launch_tile<T, 4, 2, 4>(a, st);
+  if (force == 8) return launch_tile<T, 8, 2, 4>(a, st);
+  const long long cus = a.num_cus;
+  auto tiles = [&](int rows, int cols) { return (long long)((a.M + rows - 1) / rows) * ((a.N + cols - 1) / cols); };
+  if (a.M <= 16) return tiles(16, 16) <= cus ? launch_split<T, 1, 1, 8, 4>(a, st) : launch_split<T, 1, 4, 8, 2>(a, st);
+  if (tiles(32, 32) <= cus) return launch_split<T, 2, 2, 8, 2>(a, st);
+  if (tiles(32, 64) <= 2 * cus) return launch_split<T, 2, 4, 8, 1>(a, st);
+  const long long most = cus * 9 / 16, big = tiles(256, 256);
+  if (big >= most && big * 16 >= (big + cus - 1) / cus * cus * 9) return launch_tile<T, 8, 2, 4>(a, st);
+  if (tiles(128, 256) >= most) return launch_tile<T, 4, 2, 4>(a, st);
+  if (tiles(128, 128) >= most) return launch_tile<T, 4, 2, 2>(a, st);
+  return launch_tile<T, 2, 2, 2>(a, st);
 }
 static int gemm(const Args &a, int dtype, hipStream_t st) {
   if (dtype == SOUFFLE_F16) return gemm<half_t>(a, st);
   if (dtype == SOUFFLE_BF16) return gemm<bf16_t>(a, st);
   return gemm<float>(a, st);
+}
+// Whether the product's workgroups quantise the rows themselves.
+static bool rows_in_kernel(int M, int K) {
+  const int most = getenv("SOUFFLE_ROWS") ? atoi(getenv("SOUFFLE_ROWS")) : 16384;
+  return M <= 16 && (long long)M * K <= most;
+}
+template <class T>
+static int linear_rows(const Args &a, hipStream_t st) {
+  if ((a.N + 15) / 16 <= a.num_cus) return launch_rows<T, 1, 4>(a, st);
+  return launch_rows<T, 4, 2>(a, st);
 }
 
 static int check_product(const void *packed, const float *col_scale, const void *bias, int act, const void *y, int dtype, long long ldy, int M,
@@ -636,12 +705,13 @@ extern "C" int souffle_gemm_int8(const int8_t *q, long long ldq, const float *ro
   if (reinterpret_cast<uintptr_t>(row_scale) % 4) return fail(SOUFFLE_ERR_ALIGN, "row_scale is not aligned to its elements");
   DeviceFacts df;
   if (int rc = device_facts(&df)) return rc;
-  const Args a = {q, ldq, row_scale, static_cast<const int8_t *>(packed), col_scale, bias, y, ldy, M, N, K, act, (K + 63) / 64, 0};
+  const Args a = {q, ldq, row_scale, nullptr, 0, static_cast<const int8_t *>(packed), col_scale, bias, y, ldy, M, N, K, act, (K + 63) / 64, 0, df.num_cus};
   return gemm(a, dtype, static_cast<hipStream_t>(stream));
 }
 
 extern "C" size_t souffle_linear_int8_workspace_bytes(int M, int K) {
   if (M < 0 || check_kn(K, 1)) return 0;
+  if (rows_in_kernel(M, K)) return 0;
   return round_up((size_t)M * round_up(K, 64) + (size_t)M * 4, 256);
 }
 
@@ -651,16 +721,24 @@ extern "C" int souffle_linear_int8(const void *x, long long ldx, const void *pac
   if (M == 0) return SOUFFLE_OK;
   if (!x) return fail(SOUFFLE_ERR_NULL, "x must not be NULL");
   if (int rc = check_x("x", x, dtype, ldx, K)) return rc;
-  if (!ws || ws_bytes < souffle_linear_int8_workspace_bytes(M, K))
-    return fail(SOUFFLE_ERR_WORKSPACE, "workspace too small: need %zu bytes", souffle_linear_int8_workspace_bytes(M, K));
-  if (!aligned16(ws)) return fail(SOUFFLE_ERR_ALIGN, "workspace must be 16-byte aligned");
+  const size_t need = souffle_linear_int8_workspace_bytes(M, K);
+  if (need && (!ws || ws_bytes < need)) return fail(SOUFFLE_ERR_WORKSPACE, "workspace too small: need %zu bytes", need);
+  if (need && !aligned16(ws)) return fail(SOUFFLE_ERR_ALIGN, "workspace must be 16-byte aligned");
   DeviceFacts df;
   if (int rc = device_facts(&df)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  Args a = {nullptr, 0, nullptr, x, ldx, static_cast<const int8_t *>(packed), col_scale, bias, y, ldy, M, N, K, act, (K + 63) / 64, 0, df.num_cus};
+  if (need == 0) {
+    if (dtype == SOUFFLE_F16) return linear_rows<half_t>(a, st);
+    if (dtype == SOUFFLE_BF16) return linear_rows<bf16_t>(a, st);
+    return linear_rows<float>(a, st);
+  }
   const long long ldq = (long long)round_up(K, 64);
   int8_t *q = static_cast<int8_t *>(ws);
   float *row_scale = reinterpret_cast<float *>(q + (size_t)M * ldq);
   if (int rc = quantize_rows(x, dtype, ldx, q, ldq, row_scale, M, K, st)) return rc;
-  const Args a = {q, ldq, row_scale, static_cast<const int8_t *>(packed), col_scale, bias, y, ldy, M, N, K, act, (K + 63) / 64, 0};
+  a.q = q;
+  a.ldq = ldq;
+  a.row_scale = row_scale;
   return gemm(a, dtype, st);
 }

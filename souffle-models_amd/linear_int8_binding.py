@@ -172,7 +172,7 @@ def linear_int8(x, weight, *, bias=None, act=None, out=None):
     with torch.cuda.device(dev):
         out, ldy = _output(out, M, N, x.dtype, dev)
         nbytes = sh.lib().souffle_linear_int8_workspace_bytes(M, K)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         sh.check(sh.lib().souffle_linear_int8(x.data_ptr(), ld, weight.packed.data_ptr(), weight.scale.data_ptr(), b, a, out.data_ptr(),
-                                              _DTYPES[x.dtype], ldy, M, N, K, ws.data_ptr(), nbytes, sh.current_stream()))
+                                              _DTYPES[x.dtype], ldy, M, N, K, sh.ptr(ws), nbytes, sh.current_stream()))
     return out
