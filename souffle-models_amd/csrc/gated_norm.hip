@@ -29,12 +29,12 @@ struct FwdArgs {
 template <int TPR>
 struct RowReduce {
   static constexpr int kWaves = TPR / 64;
-  unsigned *red;                    // [2][kWaves] of this row slot
+  unsigned *red;                    // [2][2 kWaves] of this row slot
   int turn;
   __device__ __forceinline__ float sum(float v) {
     v = wave_sum_dpp(v);
     if constexpr (kWaves == 1) return v;
-    float *r = reinterpret_cast<float *>(red) + turn * kWaves;
+    float *r = reinterpret_cast<float *>(red) + turn * 2 * kWaves;
     turn ^= 1;
     if ((threadIdx.x & 63) == 0) r[(threadIdx.x / 64) % kWaves] = v;
     __syncthreads();
@@ -43,10 +43,27 @@ struct RowReduce {
     for (int w = 0; w < kWaves; ++w) s += r[w];
     return s;
   }
+  // Two sums for one barrier.
+  __device__ __forceinline__ void sum2(float &v0, float &v1) {
+    v0 = wave_sum_dpp(v0);
+    v1 = wave_sum_dpp(v1);
+    if constexpr (kWaves > 1) {
+      float *r = reinterpret_cast<float *>(red) + turn * 2 * kWaves;
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0) {
+        r[(threadIdx.x / 64) % kWaves] = v0;
+        r[kWaves + (threadIdx.x / 64) % kWaves] = v1;
+      }
+      __syncthreads();
+      v0 = v1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) v0 += r[w], v1 += r[kWaves + w];
+    }
+  }
   __device__ __forceinline__ unsigned umax(unsigned v) {
     v = wave_umax_dpp(v);
     if constexpr (kWaves == 1) return v;
-    unsigned *r = red + turn * kWaves;
+    unsigned *r = red + turn * 2 * kWaves;
     turn ^= 1;
     if ((threadIdx.x & 63) == 0) r[(threadIdx.x / 64) % kWaves] = v;
     __syncthreads();
@@ -57,19 +74,19 @@ struct RowReduce {
   }
 };
 
-// The vector's elements c .. c+7, or `missing` where the caller has none.
-template <class T>
+// The vector's elements c .. c+7, or `missing` where the caller has none; zeros behind the row's end, which keep what is computed there zero.
+template <RowForm FORM, class T>
 __device__ __forceinline__ typename Vec8<T>::type param8(const void *p, int c, int n, float missing) {
-  if (p) return load8(static_cast<const T *>(p), c, n);
+  if (p) return settle_row<FORM, T>(load_row<FORM>(static_cast<const T *>(p), c, n), c, n);
   typename Vec8<T>::type v;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (T)missing;
+  for (int e = 0; e < 8; ++e) v[e] = (T)(c + e < n ? missing : 0.f);
   return v;
 }
 
 // (v - mean) / deviation or v / rms of a row in place, elements behind the row's end 0; returns 1 / deviation.  Two
 // passes over the registers: the mean first, then the squares around it, so that a large mean costs no digits.
-template <int TPR, int NV>
+template <RowForm FORM, int TPR, int NV>
 __device__ __forceinline__ float normalize(float (&v)[NV][8], int kind, float eps, int cols, int c0, RowReduce<TPR> &red) {
   const float inv_n = 1.0f / (float)cols;
   if (kind == SOUFFLE_NORM_LAYER) {
@@ -80,9 +97,17 @@ __device__ __forceinline__ float normalize(float (&v)[NV][8], int kind, float ep
       for (int e = 0; e < 8; ++e) s += v[i][e];
     const float mean = red.sum(s) * inv_n;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const float m = c0 + i * TPR * 8 < cols ? mean : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = c0 + i * TPR * 8 + e < cols ? v[i][e] - mean : 0.f;
+      for (int e = 0; e < 8; ++e) v[i][e] -= m;
+      if constexpr (FORM != kWhole) {
+        int left = cols - c0 - i * TPR * 8;
+        asm volatile("" : "+v"(left));      // (eight comparisons per row, not eight masks that are kept)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = e < left ? v[i][e] : 0.f;
+      }
+    }
   }
   float s = 0.f;
 #pragma unroll
@@ -97,23 +122,23 @@ __device__ __forceinline__ float normalize(float (&v)[NV][8], int kind, float ep
   return r;
 }
 
-template <class T, int TPR, int NV, int WG, bool OUT8>
+template <class T, int TPR, int NV, int WG, bool OUT8, RowForm FORM>
 __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
   typedef typename Vec8<T>::type V;
   constexpr int kSlots = WG / TPR;
-  __shared__ unsigned lds_red[WG / 64 * 2];
-  const int slot = threadIdx.x / TPR, t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
-  RowReduce<TPR> red{lds_red + slot * 2 * RowReduce<TPR>::kWaves, 0};
+  __shared__ __attribute__((aligned(16))) unsigned lds_red[WG / 64 * 4];
+  const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
+  RowReduce<TPR> red{lds_red + slot * 4 * RowReduce<TPR>::kWaves, 0};
 
   V pg[NV], pb[NV], gt[NV], ng[NV], nb[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + i * TPR * 8;
-    pg[i] = param8<T>(a.post_gamma, c, n, 1.f);
-    pb[i] = param8<T>(a.post_beta, c, n, 0.f);
-    ng[i] = param8<T>(a.pre_gamma, c, n, 1.f);
-    nb[i] = param8<T>(a.pre_beta, c, n, 0.f);
-    gt[i] = param8<T>(nullptr, c, n, 1.f);
+    pg[i] = param8<FORM, T>(a.post_gamma, c, n, 1.f);
+    pb[i] = param8<FORM, T>(a.post_beta, c, n, 0.f);
+    ng[i] = param8<FORM, T>(a.pre_gamma, c, n, 1.f);
+    nb[i] = param8<FORM, T>(a.pre_beta, c, n, 0.f);
+    gt[i] = param8<FORM, T>(nullptr, c, n, 1.f);
   }
   const int first = (blockIdx.x * kSlots + slot) * a.rows_per_slot, end = min(first + a.rows_per_slot, a.rows);
   int gate_row = -1;
@@ -122,8 +147,8 @@ __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
     const T *x = static_cast<const T *>(a.x) + row * a.ldx, *f = static_cast<const T *>(a.f) + row * a.ldf;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      xv[i] = load8(x, c0 + i * TPR * 8, n);
-      fv[i] = load8(f, c0 + i * TPR * 8, n);
+      xv[i] = load_row<FORM>(x, c0 + i * TPR * 8, n);
+      fv[i] = load_row<FORM>(f, c0 + i * TPR * 8, n);
     }
   };
   // (rows of several waves: one row per workgroup at a time, so every thread takes the same turns through the barriers)
@@ -134,17 +159,18 @@ __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
       if (gr != gate_row) {
         gate_row = gr;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) gt[i] = load8(static_cast<const T *>(a.gate) + (long long)gr * n, c0 + i * TPR * 8, n);
+        for (int i = 0; i < NV; ++i) gt[i] = param8<FORM, T>(static_cast<const T *>(a.gate) + (long long)gr * n, c0 + i * TPR * 8, n, 1.f);
       }
     }
     float x[NV][8], p[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      to_f32(x[i], xv[i]);
-      to_f32(p[i], fv[i]);
+      if constexpr (NV > 1) pg[i] = opaque(pg[i]), pb[i] = opaque(pb[i]), gt[i] = opaque(gt[i]), ng[i] = opaque(ng[i]), nb[i] = opaque(nb[i]);
+      to_f32(x[i], settle_row<FORM, T>(xv[i], c0 + i * TPR * 8, n));
+      to_f32(p[i], settle_row<FORM, T>(fv[i], c0 + i * TPR * 8, n));
     }
     if (row + 1 < end) fetch(row + 1);
-    if (a.post != SOUFFLE_NORM_NONE) (void)normalize<TPR, NV>(p, a.post, a.post_eps, n, c0, red);
+    if (a.post != SOUFFLE_NORM_NONE) (void)normalize<FORM, TPR, NV>(p, a.post, a.post_eps, n, c0, red);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -155,9 +181,9 @@ __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
     if (a.y) {
       T *y = static_cast<T *>(a.y) + row * a.ldy;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) store8(y, c0 + i * TPR * 8, n, from_f32<T>(x[i]));
+      for (int i = 0; i < NV; ++i) store_row<FORM>(y, c0 + i * TPR * 8, n, from_f32<T>(x[i]));
     }
-    (void)normalize<TPR, NV>(x, a.pre, a.pre_eps, n, c0, red);
+    (void)normalize<FORM, TPR, NV>(x, a.pre, a.pre_eps, n, c0, red);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -165,7 +191,7 @@ __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
     if constexpr (!OUT8) {
       T *h = static_cast<T *>(a.h) + row * a.ldh;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) store8(h, c0 + i * TPR * 8, n, from_f32<T>(x[i]));
+      for (int i = 0; i < NV; ++i) store_row<FORM>(h, c0 + i * TPR * 8, n, from_f32<T>(x[i]));
     } else {
       unsigned m = 0u;
 #pragma unroll
@@ -198,20 +224,21 @@ struct BwdArgs {
   int rows_per_gate;                // rows that share a gate row (all rows: one gate row, or no gate)
   int chunk_rows;                   // rows of a workgroup; a multiple of rows_per_gate, or within one gate row's rows
   int chunks_per_gate;              // > 0: that many chunks per gate row; 0: chunks hold whole gate rows
-  int vectors, wanted;              // wanted: bit v set = the gradient of vector v is collected
+  int vectors, wanted;              // wanted: bit v set = the gradient of vector v goes to `partial`
+  int wanted_gate;                  // the gate's gradient goes there or to dgate
   float a, post_eps, pre_eps;
 };
 
 // Several rows at a time (one per slot of TPR threads), slots in step, so that a barrier of the workgroup serves them all.
-template <class T, int TPR, int NV, int WG>
+template <class T, int TPR, int NV, int WG, RowForm FORM, bool KEEP>
 __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   typedef typename Vec8<T>::type V;
   constexpr int kSlots = WG / TPR;
-  __shared__ unsigned lds_red[WG / 64 * 2];
+  __shared__ __attribute__((aligned(16))) unsigned lds_red[WG / 64 * 4];
   __shared__ float lds_sum[kSlots > 1 ? TPR * NV * 8 : 1];
-  const int slot = threadIdx.x / TPR, t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
+  const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
   const float inv_n = 1.0f / (float)n;
-  RowReduce<TPR> red{lds_red + slot * 2 * RowReduce<TPR>::kWaves, 0};
+  RowReduce<TPR> red{lds_red + slot * 4 * RowReduce<TPR>::kWaves, 0};
 
   float sums[kVectors][NV][8] = {};
   // The slots' sums of vector v, added in the slots' order, to out[0 .. cols) by the first slot.
@@ -237,6 +264,9 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
       for (int i = 0; i < NV; ++i) store(c0 + i * TPR * 8, sums[v][i]);
   };
 
+  // a gradient that is not there: x instead, taken as zeros
+  const T *dy = static_cast<const T *>(a.dy ? a.dy : a.x), *dh = static_cast<const T *>(a.dh ? a.dh : a.x);
+  const long long ld_dy = a.dy ? a.ld_dy : a.ldx, ld_dh = a.dh ? a.ld_dh : a.ldx;
   int first, end;
   if (a.chunks_per_gate > 0) {
     const int g = blockIdx.x / a.chunks_per_gate, k = blockIdx.x % a.chunks_per_gate, g_end = min((g + 1) * a.rows_per_gate, a.rows);
@@ -250,96 +280,128 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   for (int run = first; run < end;) {
     const int gr = run / a.rows_per_gate, run_end = min((gr + 1) * a.rows_per_gate, end);
     V gt[NV], pg[NV], pb[NV], ng[NV];
+    auto vectors = [&]() {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = c0 + i * TPR * 8;
-      gt[i] = param8<T>(a.gate ? static_cast<const T *>(a.gate) + (long long)gr * n : nullptr, c, n, 1.f);
-      pg[i] = param8<T>(a.post_gamma, c, n, 1.f);
-      pb[i] = param8<T>(a.post_beta, c, n, 0.f);
-      ng[i] = param8<T>(a.pre_gamma, c, n, 1.f);
-    }
+      for (int i = 0; i < NV; ++i) {
+        const int c = c0 + i * TPR * 8;
+        gt[i] = param8<FORM, T>(a.gate ? static_cast<const T *>(a.gate) + (long long)gr * n : nullptr, c, n, 1.f);
+        pg[i] = param8<FORM, T>(a.post_gamma, c, n, 1.f);
+        pb[i] = param8<FORM, T>(a.post_beta, c, n, 0.f);
+        ng[i] = param8<FORM, T>(a.pre_gamma, c, n, 1.f);
+      }
+    };
+    vectors();
     V xv[NV], fv[NV], yv[NV], hv[NV];
     auto fetch = [&](int row) {      // (a slot without a row takes the run's first one, with gradients of zero)
       const bool valid = row < run_end;
       const long long r = valid ? row : run;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = c0 + i * TPR * 8, cd = valid ? c : n;
-        xv[i] = load8(static_cast<const T *>(a.x) + r * a.ldx, c, n);
-        fv[i] = load8(static_cast<const T *>(a.f) + r * a.ldf, c, n);
-        if (a.dy) yv[i] = load8(static_cast<const T *>(a.dy) + r * a.ld_dy, cd, n);
-        if (a.dh) hv[i] = load8(static_cast<const T *>(a.dh) + r * a.ld_dh, cd, n);
+        const int c = c0 + i * TPR * 8;
+        xv[i] = load_row<FORM>(static_cast<const T *>(a.x) + r * a.ldx, c, n);
+        fv[i] = load_row<FORM>(static_cast<const T *>(a.f) + r * a.ldf, c, n);
+        yv[i] = load_row<FORM>(dy + r * ld_dy, c, n);
+        hv[i] = load_row<FORM>(dh + r * ld_dh, c, n);
       }
     };
-    fetch(run + slot);
+    if constexpr (KEEP) fetch(run + slot);
     for (int base = run; base < run_end; base += kSlots) {
       const int row = base + slot;
       const bool valid = row < run_end;
       float y[NV][8], fh[NV][8], d[NV][8], h[NV][8];
+      if constexpr (!KEEP) {
+        fetch(row);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) pg[i] = opaque(pg[i]), pb[i] = opaque(pb[i]), gt[i] = opaque(gt[i]);
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        to_f32(y[i], xv[i]);
-        to_f32(fh[i], fv[i]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[i][e] = a.dy ? (float)yv[i][e] : 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[i][e] = a.dh ? (float)hv[i][e] : 0.f;
+        const int c = c0 + i * TPR * 8;
+        to_f32(y[i], settle_row<FORM, T>(xv[i], c, n));
+        to_f32(fh[i], settle_row<FORM, T>(fv[i], c, n));
+        to_f32(d[i], settle_row<FORM, T>(yv[i], valid && a.dy ? c : n, n));
+        to_f32(h[i], settle_row<FORM, T>(hv[i], valid && a.dh ? c : n, n));
       }
-      if (base + kSlots < run_end) fetch(row + kSlots);
+      if constexpr (KEEP)
+        if (base + kSlots < run_end) fetch(row + kSlots);
       float fr = 1.f;
-      if (a.post != SOUFFLE_NORM_NONE) fr = normalize<TPR, NV>(fh, a.post, a.post_eps, n, c0, red);
+      if (a.post != SOUFFLE_NORM_NONE) fr = normalize<FORM, TPR, NV>(fh, a.post, a.post_eps, n, c0, red);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           y[i][e] = __builtin_fmaf((float)gt[i][e], __builtin_fmaf(fh[i][e], (float)pg[i][e], (float)pb[i][e]), a.a * y[i][e]);
-      const float yr = normalize<TPR, NV>(y, a.pre, a.pre_eps, n, c0, red);
+      const float yr = normalize<FORM, TPR, NV>(y, a.pre, a.pre_eps, n, c0, red);
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (!KEEP) ng[i] = opaque(ng[i]);
+        if (a.wanted >> kPreBeta & 1)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sums[kPreBeta][i][e] += h[i][e];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           sums[kPreGamma][i][e] = __builtin_fmaf(h[i][e], y[i][e], sums[kPreGamma][i][e]);
-          sums[kPreBeta][i][e] += h[i][e];
           h[i][e] *= (float)ng[i][e];
-          s0 += h[i][e];
           s1 = __builtin_fmaf(h[i][e], y[i][e], s1);
         }
-      s0 = a.pre == SOUFFLE_NORM_LAYER ? red.sum(s0) * inv_n : 0.f;
-      s1 = red.sum(s1) * inv_n;
+        if (a.pre == SOUFFLE_NORM_LAYER)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s0 += h[i][e];
+      }
+      red.sum2(s0, s1);
+      s0 *= yr * inv_n, s1 *= yr * inv_n;
       float s2 = 0.f, s3 = 0.f;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (!KEEP) pg[i] = opaque(pg[i]), pb[i] = opaque(pb[i]), gt[i] = opaque(gt[i]);
+        if (a.pre == SOUFFLE_NORM_LAYER)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          d[i][e] = __builtin_fmaf(yr, h[i][e] - s0 - y[i][e] * s1, d[i][e]);      // gradient of y
-          sums[kGate][i][e] = __builtin_fmaf(d[i][e], __builtin_fmaf(fh[i][e], (float)pg[i][e], (float)pb[i][e]), sums[kGate][i][e]);
+          for (int e = 0; e < 8; ++e) d[i][e] -= s0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {      // gradient of y
+          d[i][e] = __builtin_fmaf(-s1, y[i][e], __builtin_fmaf(yr, h[i][e], d[i][e]));
           y[i][e] = a.a * d[i][e];
-          d[i][e] *= (float)gt[i][e];                                              // gradient of N_post(f)
-          if (!(c0 + i * TPR * 8 + e < n && valid)) d[i][e] = 0.f;
-          sums[kPostGamma][i][e] = __builtin_fmaf(d[i][e], fh[i][e], sums[kPostGamma][i][e]);
-          sums[kPostBeta][i][e] += d[i][e];
-          d[i][e] *= (float)pg[i][e];
-          s2 += d[i][e];
-          s3 = __builtin_fmaf(d[i][e], fh[i][e], s3);
         }
-      if (a.dx && valid)
+        if (a.wanted_gate)
 #pragma unroll
-        for (int i = 0; i < NV; ++i) store8(static_cast<T *>(a.dx) + row * a.ld_dx, c0 + i * TPR * 8, n, from_f32<T>(y[i]));
-      if (a.post != SOUFFLE_NORM_NONE) {
-        s2 = a.post == SOUFFLE_NORM_LAYER ? red.sum(s2) * inv_n : 0.f;
-        s3 = red.sum(s3) * inv_n;
+          for (int e = 0; e < 8; ++e)
+            sums[kGate][i][e] = __builtin_fmaf(d[i][e], __builtin_fmaf(fh[i][e], (float)pg[i][e], (float)pb[i][e]), sums[kGate][i][e]);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int e = 0; e < 8; ++e) d[i][e] *= (float)gt[i][e];      // gradient of N_post(f); the vectors are 0 behind the row's end
+        if (a.wanted >> kPostBeta & 1)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d[i][e] = fr * (d[i][e] - s2 - fh[i][e] * s3);
+          for (int e = 0; e < 8; ++e) sums[kPostBeta][i][e] += d[i][e];
+        if (a.post != SOUFFLE_NORM_NONE)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            sums[kPostGamma][i][e] = __builtin_fmaf(d[i][e], fh[i][e], sums[kPostGamma][i][e]);
+            d[i][e] *= (float)pg[i][e];
+            s3 = __builtin_fmaf(d[i][e], fh[i][e], s3);
+          }
+        if (a.post == SOUFFLE_NORM_LAYER)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s2 += d[i][e];
       }
-      if (a.df && valid)
 #pragma unroll
-        for (int i = 0; i < NV; ++i) store8(static_cast<T *>(a.df) + row * a.ld_df, c0 + i * TPR * 8, n, from_f32<T>(d[i]));
+      for (int i = 0; i < NV; ++i) store_row<FORM>(static_cast<T *>(a.dx) + row * a.ld_dx, c0 + i * TPR * 8, a.dx && valid ? n : 0, from_f32<T>(y[i]));
+      if (a.post != SOUFFLE_NORM_NONE) {
+        red.sum2(s2, s3);
+        s2 *= fr * inv_n, s3 *= fr * inv_n;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[i][e] = __builtin_fmaf(-s3, fh[i][e], fr * d[i][e]);
+          if (a.post == SOUFFLE_NORM_LAYER)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[i][e] -= s2;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store_row<FORM>(static_cast<T *>(a.df) + row * a.ld_df, c0 + i * TPR * 8, a.df && valid ? n : 0, from_f32<T>(d[i]));
     }
     if (a.dgate && a.chunks_per_gate == 0) {      // the gate row's rows were all this workgroup's
-      collect(kGate, [&](int c, const float (&v)[8]) { store8(static_cast<T *>(a.dgate) + (long long)gr * n, c, n, from_f32<T>(v)); });
+      collect(kGate, [&](int c, const float (&v)[8]) { store_row<FORM>(static_cast<T *>(a.dgate) + (long long)gr * n, c, n, from_f32<T>(v)); });
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -352,7 +414,7 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   for (int v = 0; v < kVectors; ++v)
     if (a.wanted >> v & 1) {
       float *o = out + (long long)__popc(a.wanted & ((1 << v) - 1)) * n;
-      collect(v, [&](int c, const float (&s)[8]) { store8(o, c, n, from_f32<float>(s)); });
+      collect(v, [&](int c, const float (&s)[8]) { store_row<FORM>(o, c, n, from_f32<float>(s)); });
     }
 }
 
@@ -429,25 +491,41 @@ static int check_vectors(const souffle_gated_norm_cfg *c, const souffle_gated_no
   return SOUFFLE_OK;
 }
 
-template <class T, int TPR, int NV, int WG>
+template <RowForm FORM, class T, int TPR, int NV, int WG>
 static int launch_fwd(FwdArgs a, int num_cus, hipStream_t st) {
   constexpr int kSlots = WG / TPR;
   const long long slots = (long long)num_cus * (2048 / WG) * kSlots;      // row slots that are resident at once
   a.rows_per_slot = (int)std::max<long long>(1, (a.rows + slots - 1) / slots);
   const int grid = (int)(((long long)a.rows + (long long)a.rows_per_slot * kSlots - 1) / ((long long)a.rows_per_slot * kSlots));
-  if (a.q) hipLaunchKernelGGL((k_gated_norm<T, TPR, NV, WG, true>), dim3(grid), dim3(WG), 0, st, a);
-  else hipLaunchKernelGGL((k_gated_norm<T, TPR, NV, WG, false>), dim3(grid), dim3(WG), 0, st, a);
+  if (a.q) hipLaunchKernelGGL((k_gated_norm<T, TPR, NV, WG, true, FORM>), dim3(grid), dim3(WG), 0, st, a);
+  else hipLaunchKernelGGL((k_gated_norm<T, TPR, NV, WG, false, FORM>), dim3(grid), dim3(WG), 0, st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
+template <RowForm FORM, class T>
+static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
+  // One vector of 8 per thread in fp32, two in the 16-bit types from 513 elements on (measured: 4096 x 4096 fp32 48.6 us with one
+  // and 55.5 with two, which leave two waves per SIMD; 8192 x 4096 bf16 49.3 and 45.3, where two halve the waves of a sum).
+  if constexpr (sizeof(T) == 4) {
+    if (a.cols <= 512) return launch_fwd<FORM, T, 64, 1, 256>(a, num_cus, st);
+    if (a.cols <= 1024) return launch_fwd<FORM, T, 128, 1, 128>(a, num_cus, st);
+    if (a.cols <= 2048) return launch_fwd<FORM, T, 256, 1, 256>(a, num_cus, st);
+    if (a.cols <= 4096) return launch_fwd<FORM, T, 512, 1, 512>(a, num_cus, st);
+    if (a.cols <= 8192) return launch_fwd<FORM, T, 1024, 1, 1024>(a, num_cus, st);
+    return launch_fwd<FORM, T, 1024, 2, 1024>(a, num_cus, st);
+  } else {
+    if (a.cols <= 512) return launch_fwd<FORM, T, 64, 1, 256>(a, num_cus, st);
+    if (a.cols <= 1024) return launch_fwd<FORM, T, 64, 2, 256>(a, num_cus, st);
+    if (a.cols <= 2048) return launch_fwd<FORM, T, 256, 1, 256>(a, num_cus, st);
+    if (a.cols <= 4096) return launch_fwd<FORM, T, 256, 2, 256>(a, num_cus, st);
+    if (a.cols <= 8192) return launch_fwd<FORM, T, 512, 2, 512>(a, num_cus, st);
+    return launch_fwd<FORM, T, 1024, 2, 1024>(a, num_cus, st);
+  }
+}
 template <class T>
 static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
-  if (a.cols <= 512) return launch_fwd<T, 64, 1, 256>(a, num_cus, st);
-  if (a.cols <= 1024) return launch_fwd<T, 64, 2, 256>(a, num_cus, st);
-  if (a.cols <= 2048) return launch_fwd<T, 256, 1, 256>(a, num_cus, st);
-  if (a.cols <= 4096) return launch_fwd<T, 256, 2, 256>(a, num_cus, st);
-  if (a.cols <= 8192) return launch_fwd<T, 512, 2, 512>(a, num_cus, st);
-  return launch_fwd<T, 1024, 2, 1024>(a, num_cus, st);
+  if (a.cols < 8) return launch_fwd<kShort, T, 64, 1, 256>(a, num_cus, st);
+  return a.cols % 8 ? forward<kRagged, T>(a, num_cus, st) : forward<kWhole, T>(a, num_cus, st);
 }
 
 // How the rows are cut into chunks, one workgroup each: about `want` of them, none across gate rows unless it holds
@@ -484,21 +562,25 @@ static int wanted_vectors(const souffle_gated_norm_grad *g) {
          (g->post_gamma ? 1 << kPostGamma : 0) | (g->post_beta ? 1 << kPostBeta : 0);
 }
 
-template <class T, int TPR, int NV, int WG>
+template <RowForm FORM, class T, int TPR, int NV, int WG, bool KEEP = true>
 static int launch_bwd(const BwdArgs &a, int chunks, hipStream_t st) {
-  hipLaunchKernelGGL((k_gated_norm_grad<T, TPR, NV, WG>), dim3(chunks), dim3(WG), 0, st, a);
+  hipLaunchKernelGGL((k_gated_norm_grad<T, TPR, NV, WG, FORM, KEEP>), dim3(chunks), dim3(WG), 0, st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
+template <RowForm FORM, class T>
+static int rows_backward(const BwdArgs &a, int chunks, hipStream_t st) {
+  if (a.cols <= 512) return launch_bwd<FORM, T, 64, 1, 512>(a, chunks, st);
+  if (a.cols <= 1024) return launch_bwd<FORM, T, 128, 1, 512>(a, chunks, st);
+  if (a.cols <= 2048) return launch_bwd<FORM, T, 256, 1, 512>(a, chunks, st);
+  if (a.cols <= 4096) return launch_bwd<FORM, T, 512, 1, 512>(a, chunks, st);
+  if (a.cols <= 8192) return launch_bwd<FORM, T, 512, 2, 512, false>(a, chunks, st);
+  return launch_bwd<FORM, T, 1024, 2, 1024, false>(a, chunks, st);
+}
 template <class T>
 static int backward(const BwdArgs &a, const FinishArgs &f, int gate_rows, hipStream_t st) {
-  int rc;
-  if (a.cols <= 512) rc = launch_bwd<T, 64, 1, 512>(a, f.chunks, st);
-  else if (a.cols <= 1024) rc = launch_bwd<T, 128, 1, 512>(a, f.chunks, st);
-  else if (a.cols <= 2048) rc = launch_bwd<T, 256, 1, 512>(a, f.chunks, st);
-  else if (a.cols <= 4096) rc = launch_bwd<T, 512, 1, 512>(a, f.chunks, st);
-  else if (a.cols <= 8192) rc = launch_bwd<T, 1024, 1, 1024>(a, f.chunks, st);
-  else rc = launch_bwd<T, 1024, 2, 1024>(a, f.chunks, st);
+  const int rc = a.cols < 8 ? launch_bwd<kShort, T, 64, 1, 512>(a, f.chunks, st)
+                            : a.cols % 8 ? rows_backward<kRagged, T>(a, f.chunks, st) : rows_backward<kWhole, T>(a, f.chunks, st);
   if (rc || f.vectors == 0) return rc;
   const int more = (f.wanted >> kGate & 1) ? gate_rows - 1 : 0;
   hipLaunchKernelGGL(k_gated_norm_grad_finish<T>, dim3((a.cols + 63) / 64, f.vectors + more), dim3(1024), 0, st, f);
@@ -597,6 +679,7 @@ extern "C" int souffle_gated_norm_backward(const souffle_gated_norm_cfg *c, cons
   a.rows_per_gate = rpg; a.chunk_rows = ch.rows; a.chunks_per_gate = ch.per_gate;
   a.wanted = gate_direct ? wanted & ~(1 << kGate) : wanted;
   a.vectors = __builtin_popcount(a.wanted);
+  a.wanted_gate = g->gate != nullptr;
   a.a = c->residual_scale; a.post_eps = c->post_eps; a.pre_eps = c->pre_eps;
   FinishArgs fin = {static_cast<const float *>(ws), {g->pre_gamma, g->pre_beta, g->gate, g->post_gamma, g->post_beta}, c->cols, a.vectors, a.wanted, ch.count, ch.per_gate};
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -40,7 +40,7 @@ __device__ __forceinline__ i4 ldg16(const int8_t *p) { return *(const __attribut
 // ---------------------------------------------------------------------------------------- quantisation ----
 // Rows: TPR threads per row, NV vectors of 8 per thread kept in registers between the largest value and the rounding
 // (NV = 0: any length, the row is read again for the rounding).  Bound by memory: 3 bytes per fp16 element.
-template <class T, int TPR, int NV>
+template <class T, int TPR, int NV, RowForm FORM>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T *x, long long ldx, int8_t *q, long long ldq, float *scale, int rows, int cols) {
   constexpr int kSlots = 256 / TPR;
   __shared__ unsigned lds_max[4];
@@ -51,19 +51,25 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T *x, long long ldx
   int8_t *qr = q + row * ldq;
   typename Vec8<T>::type v[NV ? NV : 1];
   unsigned m = 0u;
-  auto widen = [&](typename Vec8<T>::type w) {
-    float f[8];
-    to_f32(f, w);
+  auto widen = [&](float (&f)[8], typename Vec8<T>::type w, int c) { to_f32(f, settle_row<FORM, T>(w, c, cols)); };
+  auto largest = [&](const float (&f)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
   };
+  float f[NV ? NV : 1][8];
   if constexpr (NV > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = load8(xr, (i * TPR + t) * 8, cols);
+    for (int i = 0; i < NV; ++i) v[i] = load_row<FORM>(xr, (i * TPR + t) * 8, cols);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) widen(v[i]);
+    for (int i = 0; i < NV; ++i) {
+      widen(f[i], v[i], (i * TPR + t) * 8);
+      largest(f[i]);
+    }
   } else {
-    for (int c = t * 8; c < cols; c += TPR * 8) widen(load8(xr, c, cols));
+    for (int c = t * 8; c < cols; c += TPR * 8) {
+      widen(f[0], load_row<FORM>(xr, c, cols), c);
+      largest(f[0]);
+    }
   }
   m = wave_umax_dpp(m);
   if constexpr (TPR > 64) {
@@ -72,16 +78,18 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T *x, long long ldx
     m = max(max(lds_max[0], lds_max[1]), max(lds_max[2], lds_max[3]));
   }
   const RowScale rs = row_scale(m);
-  auto put = [&](typename Vec8<T>::type w, int c) {
-    float f[8];
-    to_f32(f, w);
-    if (c < cols) *reinterpret_cast<u2 *>(qr + c) = quantize8(f, rs);
-  };
   if constexpr (NV > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) put(v[i], (i * TPR + t) * 8);
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * 8;
+      const u2 p = quantize8(f[i], rs);
+      if (c < cols) *reinterpret_cast<u2 *>(qr + c) = p;
+    }
   } else {
-    for (int c = t * 8; c < cols; c += TPR * 8) put(load8(xr, c, cols), c);
+    for (int c = t * 8; c < cols; c += TPR * 8) {
+      widen(f[0], load_row<FORM>(xr, c, cols), c);
+      *reinterpret_cast<u2 *>(qr + c) = quantize8(f[0], rs);
+    }
   }
   if (t == 0) scale[row] = rs.scale;
 }
@@ -236,11 +244,22 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
     for (int base = 0, turn = 0; base < a.M; base += slots, turn ^= 1) {
       const int row = base + wave / per_row;
       const T *x = static_cast<const T *>(a.x) + min(row, a.M - 1) * a.ldx;
-      typename Vec8<T>::type first = load8(x, c0, a.K);
+      auto values = [&](float (&f)[8], int c) {
+        if (a.K % 8 == 0) to_f32(f, settle_row<kWhole, T>(load_row<kWhole>(x, c, a.K), c, a.K));
+        else if (a.K > 8) to_f32(f, settle_row<kRagged, T>(load_row<kRagged>(x, c, a.K), c, a.K));
+        else to_f32(f, settle_row<kShort, T>(load_row<kShort>(x, c, a.K), c, a.K));
+      };
+      float first[8];
+      values(first, c0);
       float f[8];
       unsigned m = 0u;
       for (int c = c0; c < a.K; c += stride) {
-        to_f32(f, c == c0 ? first : load8(x, c, a.K));
+        if (c == c0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = max(m, abs_bits(first[e]));
+          continue;
+        }
+        values(f, c);
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
       }
@@ -251,8 +270,8 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
       const RowScale rs = row_scale(m);
       if (row < a.M) {
         for (int c = c0; c < a.K; c += stride) {
-          to_f32(f, c == c0 ? first : load8(x, c, a.K));
-          *reinterpret_cast<u2 *>(lds_rows + row * pitch + c) = quantize8(f, rs);
+          if (c != c0) values(f, c);
+          *reinterpret_cast<u2 *>(lds_rows + row * pitch + c) = quantize8(c == c0 ? first : f, rs);
         }
         if (lane == 0) lds_scale[row] = rs.scale;
       }
@@ -522,16 +541,22 @@ static int check_x(const char *name, const void *x, int dtype, long long ld, int
   return SOUFFLE_OK;
 }
 
+template <RowForm FORM, class T>
+static void launch_quantize(const T *x, long long ldx, int8_t *q, long long ldq, float *scale, int M, int K, hipStream_t st) {
+  const dim3 wide(M), narrow((M + 3) / 4), block(256);
+  if (K <= 512) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1, FORM>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 1024) hipLaunchKernelGGL((k_quantize_rows<T, 64, 2, FORM>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 2048) hipLaunchKernelGGL((k_quantize_rows<T, 256, 1, FORM>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 4096) hipLaunchKernelGGL((k_quantize_rows<T, 256, 2, FORM>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 8192) hipLaunchKernelGGL((k_quantize_rows<T, 256, 4, FORM>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else hipLaunchKernelGGL((k_quantize_rows<T, 256, 0, FORM>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+}
 template <class T>
 static int quantize_rows(const void *xv, long long ldx, int8_t *q, long long ldq, float *scale, int M, int K, hipStream_t st) {
   const T *x = static_cast<const T *>(xv);
-  const dim3 wide(M), narrow((M + 3) / 4), block(256);
-  if (K <= 512) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
-  else if (K <= 1024) hipLaunchKernelGGL((k_quantize_rows<T, 64, 2>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
-  else if (K <= 2048) hipLaunchKernelGGL((k_quantize_rows<T, 256, 1>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
-  else if (K <= 4096) hipLaunchKernelGGL((k_quantize_rows<T, 256, 2>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
-  else if (K <= 8192) hipLaunchKernelGGL((k_quantize_rows<T, 256, 4>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
-  else hipLaunchKernelGGL((k_quantize_rows<T, 256, 0>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  if (K < 8) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1, kShort>), dim3((M + 3) / 4), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K % 8) launch_quantize<kRagged>(x, ldx, q, ldq, scale, M, K, st);
+  else launch_quantize<kWhole>(x, ldx, q, ldq, scale, M, K, st);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }

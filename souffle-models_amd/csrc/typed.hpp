@@ -16,7 +16,57 @@ struct Vec8 {
   typedef T unaligned __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
-// Elements c .. c+7 of a row of n; what lies behind the row's end reads as zero.
+// How the length n of a row goes into vectors: a multiple of 8, with a rest, or shorter than one vector.
+enum RowForm { kWhole = 0, kRagged = 1, kShort = 2 };
+// Elements c .. c+7 of a row of n, in two steps that both run without a branch around the load: load_row takes the eight
+// elements from min(c, n - 8) on (all lanes load, also those behind the row's end), and settle_row, where the data is used, moves the
+// row's last elements into place and zeroes what lies behind it.  (A lane that skips a load by a branch makes
+// the whole wave wait for every load it has in flight, at each such branch.)
+template <RowForm FORM, class T>
+__device__ __forceinline__ typename Vec8<T>::type load_row(const T *row, int c, int n) {
+  if constexpr (FORM != kShort) {
+    return *(const __attribute__((address_space(1))) typename Vec8<T>::unaligned *)(row + min(c, n - 8));
+  } else {
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = *(const __attribute__((address_space(1))) T *)(row + min(c + e, n - 1));
+    return v;
+  }
+}
+template <RowForm FORM, class T>
+__device__ __forceinline__ typename Vec8<T>::type settle_row(typename Vec8<T>::type v, int c, int n) {
+  if constexpr (FORM != kShort) {
+    constexpr int kWords = sizeof(T) * 2, kHalf = sizeof(T) == 2;      // 32-bit words of a vector; two elements a word
+    typedef unsigned W __attribute__((ext_vector_type(kWords)));
+    W w = __builtin_bit_cast(W, v);
+    if constexpr (FORM == kRagged) {
+      const int by = c - min(c, n - 8);      // elements to move down
+#pragma unroll
+      for (int step = 4; step >= 1; step >>= 1) {
+        const bool on = by & step;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          unsigned moved;
+          if (kHalf && step == 1) {
+            moved = i + 1 < kWords ? __builtin_amdgcn_alignbit(w[i + 1 < kWords ? i + 1 : i], w[i], 16) : w[i] >> 16;
+          } else {
+            const int d = kHalf ? step / 2 : step;
+            moved = i + d < kWords ? w[i + d < kWords ? i + d : i] : 0u;
+          }
+          w[i] = on ? moved : w[i];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = c < n ? w[i] : 0u;
+    return __builtin_bit_cast(typename Vec8<T>::type, w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < n ? v[e] : (T)0.f;
+    return v;
+  }
+}
+// The same at once, for a lane that may be the only one with something to load.
 template <class T>
 __device__ __forceinline__ typename Vec8<T>::type load8(const T *row, int c, int n) {
   typedef typename Vec8<T>::type V;
@@ -27,15 +77,24 @@ __device__ __forceinline__ typename Vec8<T>::type load8(const T *row, int c, int
     if (c + e < n) v[e] = *(const __attribute__((address_space(1))) T *)(row + c + e);
   return v;
 }
-template <class T>
-__device__ __forceinline__ void store8(T *row, int c, int n, typename Vec8<T>::type v) {
-  if (c + 8 <= n) {
-    *(__attribute__((address_space(1))) typename Vec8<T>::unaligned *)(row + c) = v;
-    return;
-  }
+template <RowForm FORM, class T>
+__device__ __forceinline__ void store_row(T *row, int c, int n, typename Vec8<T>::type v) {
+  if (c + 8 <= n) *(__attribute__((address_space(1))) typename Vec8<T>::unaligned *)(row + c) = v;
+  if constexpr (FORM != kWhole)
+    if (c + 8 > n)
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (c + e < n) *(__attribute__((address_space(1))) T *)(row + c + e) = v[e];
+      for (int e = 0; e < 7; ++e)
+        if (c + e < n) *(__attribute__((address_space(1))) T *)(row + c + e) = v[e];
+}
+// The vector as a value that the optimiser cannot see through: what is computed from it in a loop stays there (conversions of
+// a loop's constants to fp32, moved out of it, take twice the registers of the constants).
+template <class V>
+__device__ __forceinline__ V opaque(V v) {
+  typedef unsigned W __attribute__((ext_vector_type(sizeof(V) / 4)));
+  W w = __builtin_bit_cast(W, v);
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(V) / 4); ++i) asm volatile("" : "+v"(w[i]));
+  return __builtin_bit_cast(V, w);
 }
 template <class V>
 __device__ __forceinline__ void to_f32(float (&f)[8], V v) {
