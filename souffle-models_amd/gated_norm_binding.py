@@ -45,11 +45,31 @@ def _on_device(position):
     return decorate
 
 
-def _check_vector(name, v, x, D, index, rows_too=False):
-    _check_cuda(name, v, index)
-    if v.dtype != x.dtype or not v.is_contiguous() or v.shape[-1:] != (D,) or not (v.dim() == 1 or (rows_too and v.dim() == 2)):
-        raise ValueError("%s must be contiguous, of x's type and %s" % (name, "[%d] or [G, %d]" % (D, D) if rows_too else "[%d]" % D))
+def _vector(name, v, x, D, index):
+    """Address of a vector [D] of x's type, or None."""
+    if v is None:
+        return None
+    if not isinstance(v, torch.Tensor) or v.get_device() != index or v.dtype is not x.dtype or v.shape != (D,) or not v.is_contiguous():
+        _check_cuda(name, v, index)
+        raise ValueError("%s must be contiguous, of x's type and [%d]" % (name, D))
     return v.data_ptr()
+
+
+def _gate(gate, x, M, D, index):
+    """(address of a gate [D] or [G, D], rows that share one of its rows; 0: all)."""
+    if gate is None or not isinstance(gate, torch.Tensor) or gate.dim() != 2:
+        return _vector("gate", gate, x, D, index), 0
+    G = gate.shape[0]
+    if G < 1 or M % G:
+        raise ValueError("a gate of %d rows does not divide %d rows" % (G, M))
+    if gate.get_device() != index or gate.dtype is not x.dtype or gate.shape[1] != D or not gate.is_contiguous():
+        _check_cuda("gate", gate, index)
+        raise ValueError("gate must be contiguous, of x's type and [%d] or [G, %d]" % (D, D))
+    return gate.data_ptr(), M // G
+
+
+def _like(x):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_eps, pre_norm, pre_gamma, pre_beta, pre_eps):
@@ -66,19 +86,11 @@ def _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_ep
     x, ldx = _rows("x", x)
     f, ldf = _rows("f", f)
     M, D = x.shape
-    per_gate = 0
-    gate_ptr = None
-    if gate is not None:
-        gate_ptr = _check_vector("gate", gate, x, D, index, True)
-        if gate.dim() == 2:
-            if gate.shape[0] < 1 or M % gate.shape[0]:
-                raise ValueError("a gate of %d rows does not divide %d rows" % (gate.shape[0], M))
-            per_gate = M // gate.shape[0]
+    gate_ptr, per_gate = _gate(gate, x, M, D, index)
     if post_norm is None and (post_gamma is not None or post_beta is not None):
         raise ValueError("post_gamma and post_beta need a post_norm")
-    vector = lambda name, v: None if v is None else _check_vector(name, v, x, D, index)  # noqa: E731
-    w = sh.GatedNormW(vector("post_gamma", post_gamma), vector("post_beta", post_beta), gate_ptr, vector("pre_gamma", pre_gamma),
-                      vector("pre_beta", pre_beta))
+    w = sh.GatedNormW(_vector("post_gamma", post_gamma, x, D, index), _vector("post_beta", post_beta, x, D, index), gate_ptr,
+                      _vector("pre_gamma", pre_gamma, x, D, index), _vector("pre_beta", pre_beta, x, D, index))
     cfg = _cfg(M, D, _DTYPES[dtype], _NORMS[post_norm], _NORMS[pre_norm], per_gate, float(residual_scale), float(post_eps), float(pre_eps), ldx, ldf, D, D)
     return x, f, index, cfg, w
 
@@ -88,8 +100,8 @@ def gated_norm(x, f, *, gate=None, residual_scale=1.0, post_norm="layer", post_g
                pre_norm="layer", pre_gamma=None, pre_beta=None, pre_eps=1e-5, want_y=True):
     """(y, h), of x's shape and type; y is None with want_y=False (a post-norm encoder only keeps h)."""
     xr, fr, index, cfg, w = _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_eps, pre_norm, pre_gamma, pre_beta, pre_eps)
-    y = x.new_empty(x.shape) if want_y else None
-    h = x.new_empty(x.shape)
+    y = _like(x) if want_y else None
+    h = _like(x)
     sh.check(sh.lib().souffle_gated_norm_forward(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), h.data_ptr(), sh.stream_of(index)))
     return y, h
 
@@ -102,7 +114,7 @@ def gated_norm_int8(x, f, *, gate=None, residual_scale=1.0, post_norm="layer", p
     xr, fr, index, cfg, w = _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_eps, pre_norm, pre_gamma, pre_beta, pre_eps)
     M, D = xr.shape
     ldq = -(-D // 64) * 64
-    y = x.new_empty(x.shape) if want_y else None
+    y = _like(x) if want_y else None
     q = x.new_empty((M, ldq), dtype=torch.int8)
     scale = x.new_empty(M, dtype=torch.float32)
     sh.check(sh.lib().souffle_gated_norm_forward_int8(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), q.data_ptr(), ldq, scale.data_ptr(),
@@ -130,9 +142,12 @@ def gated_norm_backward(dy, dh, x, f, *, gate=None, residual_scale=1.0, post_nor
             raise ValueError("%s must have x's shape and type" % name)
         d, ld = _rows(name, d)
         incoming.append((d.data_ptr(), ld))
-    g = {"x": x.new_empty(x.shape), "f": x.new_empty(x.shape)}
-    for name, v in (("gate", gate), ("post_gamma", post_gamma), ("post_beta", post_beta), ("pre_gamma", pre_gamma), ("pre_beta", pre_beta)):
-        g[name] = None if v is None else v.new_empty(v.shape) if M else v.new_zeros(v.shape)
+    given = [n for n, v in (("post_gamma", post_gamma), ("post_beta", post_beta), ("pre_gamma", pre_gamma), ("pre_beta", pre_beta)) if v is not None]
+    vectors = x.new_empty((len(given), D)) if M else x.new_zeros((len(given), D))      # (one allocation: each takes as long as a check of all)
+    g = {"x": _like(x), "f": _like(x), "gate": None, "post_gamma": None, "post_beta": None, "pre_gamma": None, "pre_beta": None}
+    g.update(zip(given, vectors.unbind(0)))
+    if gate is not None:
+        g["gate"] = gate.new_empty(gate.shape) if M else gate.new_zeros(gate.shape)
     if M == 0:
         return g
     (dy_ptr, ld_dy), (dh_ptr, ld_dh) = incoming
