@@ -14,7 +14,6 @@
 // bytes of an fp16 result.
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 #include "typed.hpp"
 #include "host_util.hpp"
 
@@ -202,7 +201,8 @@ __device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s, float
 // lines of the rows.
 //
 // ROWS: the rows come as activations, and every workgroup quantises all of them into LDS itself while its first weights
-// are under way: for a few rows that costs less than a launch of its own in front of this one.
+// are under way: for a few rows that costs less than a launch of its own in front of this one.  (Not for the 32 rows of a wider
+// tile: 384 x 768 -> 768 takes 8.2 us that way and 6.6 in two launches; twelve workgroups repeat each row's work.)
 template <class T, int MF, int NF, int W, int U, bool ROWS>
 __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
   static_assert(4 % NF == 0, "operands of the four that 64 columns have");
@@ -249,29 +249,28 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
         else if (a.K > 8) to_f32(f, settle_row<kRagged, T>(load_row<kRagged>(x, c, a.K), c, a.K));
         else to_f32(f, settle_row<kShort, T>(load_row<kShort>(x, c, a.K), c, a.K));
       };
-      float first[8];
+      float first[8], f[8];
       values(first, c0);
-      float f[8];
       unsigned m = 0u;
-      for (int c = c0; c < a.K; c += stride) {
-        if (c == c0) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) m = max(m, abs_bits(first[e]));
-          continue;
-        }
+      for (int e = 0; e < 8; ++e) m = max(m, abs_bits(first[e]));
+      for (int c = c0 + stride; c < a.K; c += stride) {
         values(f, c);
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
       }
       m = wave_umax_dpp(m);
-      if (lane == 0) lds_max[turn][wave] = m;
-      __syncthreads();
-      for (int w = 0; w < per_row; ++w) m = max(m, lds_max[turn][wave / per_row * per_row + w]);
+      if (per_row > 1) {
+        if (lane == 0) lds_max[turn][wave] = m;
+        __syncthreads();
+        for (int w = 0; w < per_row; ++w) m = max(m, lds_max[turn][wave / per_row * per_row + w]);
+      }
       const RowScale rs = row_scale(m);
       if (row < a.M) {
-        for (int c = c0; c < a.K; c += stride) {
-          if (c != c0) values(f, c);
-          *reinterpret_cast<u2 *>(lds_rows + row * pitch + c) = quantize8(c == c0 ? first : f, rs);
+        if (c0 < a.K) *reinterpret_cast<u2 *>(lds_rows + row * pitch + c0) = quantize8(first, rs);
+        for (int c = c0 + stride; c < a.K; c += stride) {
+          values(f, c);
+          *reinterpret_cast<u2 *>(lds_rows + row * pitch + c) = quantize8(f, rs);
         }
         if (lane == 0) lds_scale[row] = rs.scale;
       }
@@ -610,43 +609,38 @@ static int launch_tile(Args a, hipStream_t st) {
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
+static long long tiles(int M, int rows, int N, int cols) { return (long long)((M + rows - 1) / rows) * ((N + cols - 1) / cols); }
+
+// Which kernel: the one with the most work per workgroup that still gives the CUs enough workgroups.  Measured alone on the GPU (bf16
+// out, us; split = 32 x 32 / 32 x 64 with the waves along K, tiles of 64 x 128 with four waves | with two | 128 x 128 | 256 x 256):
+//   64 x 4096 x 4096      7.5 /  8.3   15.3 | 17.4 | 21.0 | 44.7       512 x 4096 x 4096    39 / 25   16.3 | 18.3 | 21.8 | 48.2
+//   384 x 768 x 768       4.3 /  3.7    5.7 |  6.6 |  7.8 | 15.2       1024 x 768 x 2304    15 / 10    8.4 |  8.2 |  7.8 | 14.5
+//   8192 x 768 x 2304      99 /   62   30.1 | 26.5 | 26.7 | 30.2       5760 x 1600 x 1925   85 / 63   43.5 | 37.3 | 33.6 | 32.7
+//   8192 x 4096 x 4096    315 (per 64 x 64)  184 | 149 | 142 | 112     (288 tiles of 256 x 256 on 256 CUs: the second round is an eighth full)
 template <class T>
 static int gemm(const Args &a, hipStream_t st) {
-  const int force = getenv("SOUFFLE_TILE") ? atoi(getenv("SOUFFLE_TILE")) : -1;
-  if (force == 0) return launch_split<T, 1, 1, 8, 4>(a, st);
-  if (force == 1) return launch_split<T, 1, 4, 8, 2>(a, st);
-  if (force == 2) return launch_split<T, 2, 2, 8, 2>(a, st);
-  if (force == 3) return launch_split<T, 2, 4, 8, 1>(a, st);
-  if (force == 4) return launch_tile<T, 2, 2, 2>(a, st);
-  if (force == 5) return launch_tile<T, 4, 1, 2>(a, st);
-  if (force == 6) return launch_tile<T, 4, 2, 2>(a, st);
-  if (force == 7) return launch_tile<T, 4, 2, 4>(a, st);
-  if (force == 8) return launch_tile<T, 8, 2, 4>(a, st);
-  const long long cus = a.num_cus;
-  auto tiles = [&](int rows, int cols) { return (long long)((a.M + rows - 1) / rows) * ((a.N + cols - 1) / cols); };
-  if (a.M <= 16) return tiles(16, 16) <= cus ? launch_split<T, 1, 1, 8, 4>(a, st) : launch_split<T, 1, 4, 8, 2>(a, st);
-  if (tiles(32, 32) <= cus) return launch_split<T, 2, 2, 8, 2>(a, st);
-  if (tiles(32, 64) <= 2 * cus) return launch_split<T, 2, 4, 8, 1>(a, st);
-  const long long most = cus * 9 / 16, big = tiles(256, 256);
-  if (big >= most && big * 16 >= (big + cus - 1) / cus * cus * 9) return launch_tile<T, 8, 2, 4>(a, st);
-  if (tiles(128, 256) >= most) return launch_tile<T, 4, 2, 4>(a, st);
-  if (tiles(128, 128) >= most) return launch_tile<T, 4, 2, 2>(a, st);
-  return launch_tile<T, 2, 2, 2>(a, st);
+  const long long cus = a.num_cus, big = tiles(a.M, 256, a.N, 256), rounds = (big + cus - 1) / cus;
+  if (a.M <= 16) return tiles(a.M, 16, a.N, 16) <= cus ? launch_split<T, 1, 1, 8, 4>(a, st) : launch_split<T, 1, 4, 8, 2>(a, st);
+  if (tiles(a.M, 32, a.N, 32) <= cus) return launch_split<T, 2, 2, 8, 2>(a, st);
+  if (tiles(a.M, 32, a.N, 64) <= 2 * cus) return launch_split<T, 2, 4, 8, 1>(a, st);
+  if (tiles(a.M, 64, a.N, 128) <= cus) return launch_tile<T, 2, 2, 2>(a, st);
+  if (rounds == 1 ? big * 16 >= cus * 9 : big * 10 >= rounds * cus * 7) return launch_tile<T, 8, 2, 4>(a, st);
+  return a.K >= 1536 ? launch_tile<T, 4, 2, 2>(a, st) : launch_tile<T, 4, 1, 2>(a, st);
 }
 static int gemm(const Args &a, int dtype, hipStream_t st) {
   if (dtype == SOUFFLE_F16) return gemm<half_t>(a, st);
   if (dtype == SOUFFLE_BF16) return gemm<bf16_t>(a, st);
   return gemm<float>(a, st);
 }
-// Whether the product's workgroups quantise the rows themselves.
+// Whether the product's workgroups quantise the rows themselves (one launch, no workspace): measured in one launch and in two, us,
+// 1 x 768 -> 2304 3.7 and 5.0, 2 x 4096 -> 8192 9.1 and 10.1, 4 x 4096 -> 4096 9.0 and 8.9, 8 x 4096 -> 4096 11.5 and 9.2, 16 x 1024 -> 4096
+// 6.0 and 6.0 (and some 4 us less on the host).
 static bool rows_in_kernel(int M, int K) {
-  const int most = getenv("SOUFFLE_ROWS") ? atoi(getenv("SOUFFLE_ROWS")) : 16384;
-  return M <= 16 && (long long)M * K <= most;
+  return M <= 16 && (long long)M * K <= 16384;
 }
 template <class T>
 static int linear_rows(const Args &a, hipStream_t st) {
-  if ((a.N + 15) / 16 <= a.num_cus) return launch_rows<T, 1, 4>(a, st);
-  return launch_rows<T, 4, 2>(a, st);
+  return tiles(a.M, 16, a.N, 16) <= a.num_cus ? launch_rows<T, 1, 4>(a, st) : launch_rows<T, 4, 2>(a, st);
 }
 
 static int check_product(const void *packed, const float *col_scale, const void *bias, int act, const void *y, int dtype, long long ldy, int M,
@@ -734,9 +728,8 @@ extern "C" int souffle_gemm_int8(const int8_t *q, long long ldq, const float *ro
   return gemm(a, dtype, static_cast<hipStream_t>(stream));
 }
 
-extern "C" size_t souffle_linear_int8_workspace_bytes(int M, int K) {
-  if (M < 0 || check_kn(K, 1)) return 0;
-  if (rows_in_kernel(M, K)) return 0;
+extern "C" size_t souffle_linear_int8_workspace_bytes(int M, int N, int K) {
+  if (M < 0 || check_kn(K, N) || rows_in_kernel(M, K)) return 0;
   return round_up((size_t)M * round_up(K, 64) + (size_t)M * 4, 256);
 }
 
@@ -746,7 +739,7 @@ extern "C" int souffle_linear_int8(const void *x, long long ldx, const void *pac
   if (M == 0) return SOUFFLE_OK;
   if (!x) return fail(SOUFFLE_ERR_NULL, "x must not be NULL");
   if (int rc = check_x("x", x, dtype, ldx, K)) return rc;
-  const size_t need = souffle_linear_int8_workspace_bytes(M, K);
+  const size_t need = souffle_linear_int8_workspace_bytes(M, N, K);
   if (need && (!ws || ws_bytes < need)) return fail(SOUFFLE_ERR_WORKSPACE, "workspace too small: need %zu bytes", need);
   if (need && !aligned16(ws)) return fail(SOUFFLE_ERR_ALIGN, "workspace must be 16-byte aligned");
   DeviceFacts df;

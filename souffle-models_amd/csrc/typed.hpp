@@ -158,23 +158,29 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
   return r;
 }
 // The rounding is that of the real quotient, not of a rounded one: halves are common (any value that is half its row's
-// largest is 63.5 s), and a product in fp32 would fall on either side of them.  t = x * (1/s) is off by less than 2^-16, so q0 = rint(t)
-// is right unless t lies within that of a half; there e = x - q0 s decides, which the fused multiply-add gives exactly
-// (x and q0 s are multiples of a power of two that |e| <= s holds fewer than 2^24 of).
-__device__ __forceinline__ int quantize(float x, const RowScale &r) {
-  const float t = x * r.inverse;
-  float q = __builtin_rintf(t);
-  if (__builtin_fabsf(t - q) > 0.4998f) {
-    const float e = __builtin_fmaf(-q, r.scale, x), half = 0.5f * r.scale;
-    if (e > half || (e == half && ((int)q & 1))) q += 1.0f;
-    else if (e < -half || (e == -half && ((int)q & 1))) q -= 1.0f;
-  }
-  return r.finite ? (int)q : 0;
+// largest is 63.5 s), and a product in fp32 would fall on either side of them.  Added to 1.5 * 2^23 in a fused multiply-add, x times
+// 1/s is rounded to a whole number q that stands in the sum's low bits in two's complement; it is off by one at most, and
+// e = x - q s, which the second fused multiply-add gives exactly (x and q s are multiples of a power of two that
+// |e| <= s holds fewer than 2^24 of), says where: beyond half a step, or at half a step from an odd q.
+__device__ __forceinline__ unsigned quantize_bits(float x, const RowScale &r) {      // the low byte counts
+  constexpr float kShift = 12582912.0f;
+  const float sum = __builtin_fmaf(x, r.inverse, kShift);
+  const unsigned bits = __builtin_bit_cast(unsigned, sum);
+  const float e = __builtin_fmaf(kShift - sum, r.scale, x);
+  const float half = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, 0.5f * r.scale) - (bits & 1u));      // odd: the next number below, so that half a step itself is beyond it
+  return bits + (e > half ? 1u : 0u) - (e < -half ? 1u : 0u);
 }
+__device__ __forceinline__ int quantize(float x, const RowScale &r) { return r.finite ? (int)(int8_t)quantize_bits(x, r) : 0; }
 __device__ __forceinline__ u2 quantize8(const float (&f)[8], const RowScale &r) {
-  u2 p = {0u, 0u};
+  u2 p;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) p[e >> 2] |= ((unsigned)quantize(f[e], r) & 255u) << (8 * (e & 3));
+  for (int h = 0; h < 2; ++h) {
+    unsigned b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = quantize_bits(f[4 * h + e], r);
+    const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    p[h] = r.finite ? lo | hi : 0u;
+  }
   return p;
 }
 

@@ -180,7 +180,7 @@ def linear_int8(x, weight, *, bias=None, act=None, out=None):
     b, a = _epilogue(bias, act, N, x.dtype, index)
     out, ldy = _output(out, x, M, N, x.dtype, index)
     lib = sh.lib()
-    nbytes = lib.souffle_linear_int8_workspace_bytes(M, K)
+    nbytes = lib.souffle_linear_int8_workspace_bytes(M, N, K)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     sh.check(lib.souffle_linear_int8(x.data_ptr(), ld, packed, scale, b, a, out.data_ptr(), _DTYPES[x.dtype], ldy, M, N, K, sh.ptr(ws), nbytes,
                                      sh.stream_of(index)))

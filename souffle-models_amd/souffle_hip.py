@@ -153,7 +153,7 @@ SIGNATURES = {
                                         C.c_void_p]),
     "souffle_gemm_int8": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
                                     C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p]),
-    "souffle_linear_int8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "souffle_linear_int8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "souffle_linear_int8": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
                                       C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "souffle_gated_norm_forward": (C.c_int, [C.POINTER(GatedNormCfg), C.POINTER(GatedNormW), C.c_void_p, C.c_void_p, C.c_void_p,

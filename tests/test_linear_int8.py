@@ -45,7 +45,7 @@ def test_refusals_without_gpu():
     assert lib.souffle_int8_packed_bytes(100, 65) == 128 * 128
     assert lib.souffle_int8_packed_bytes(0, 64) == 0 and "K must be" in sh.last_error()
     assert lib.souffle_int8_packed_bytes(131072, 64) == 0 and lib.souffle_int8_packed_bytes(131071, 64) == 131072 * 64
-    assert lib.souffle_linear_int8_workspace_bytes(300, 100) >= 300 * 132 and lib.souffle_linear_int8_workspace_bytes(-1, 100) == 0
+    assert lib.souffle_linear_int8_workspace_bytes(300, 8000, 1100) >= 300 * (1152 + 4) and lib.souffle_linear_int8_workspace_bytes(-1, 64, 100) == 0
     q = lambda **k: lib.souffle_quantize_rows(*{**dict(x=P, t=0, ldx=100, q=P, ldq=128, s=P, M=2, K=100, st=None), **k}.values())  # noqa: E731
     assert q(x=None) == -1 and q(q=None) == -1 and q(s=None) == -1
     assert q(t=3) == -2 and "dtype" in sh.last_error()
@@ -58,9 +58,9 @@ def test_refusals_without_gpu():
     assert g(act=4) == -2 and "activation" in sh.last_error()
     assert g(t=-1) == -2 and g(ldy=49) == -2 and g(ldq=64) == -2 and g(N=0) == -2 and g(K=131072) == -2 and g(M=-1) == -2
     assert g(ldq=136) == -3 and g(w=P + 8) == -3 and g(b=P + 1) == -3 and g(y=P + 1) == -3 and g(M=0, q=None, y=None) == 0
-    l = lambda **k: lib.souffle_linear_int8(*{**dict(x=P, ldx=100, w=P, cs=P, b=None, act=3, y=P, t=2, ldy=50, M=200, N=50, K=100, ws=P, n=1 << 20, st=None), **k}.values())  # noqa: E731
+    l = lambda **k: lib.souffle_linear_int8(*{**dict(x=P, ldx=2000, w=P, cs=P, b=None, act=3, y=P, t=2, ldy=50, M=200, N=50, K=2000, ws=P, n=1 << 20, st=None), **k}.values())  # noqa: E731
     assert l(ws=None) == -4 and l(n=100) == -4 and "workspace" in sh.last_error()
-    assert l(x=None) == -1 and l(ldx=99) == -2 and l(x=P + 2) == -3 and l(ws=P + 4) == -3 and l(M=0, ws=None, n=0) == 0
+    assert l(x=None) == -1 and l(ldx=1999) == -2 and l(x=P + 2) == -3 and l(ws=P + 4) == -3 and l(M=0, ws=None, n=0) == 0
     p = lambda **k: lib.souffle_int8_pack_weight(*{**dict(w=P, ldw=50, p=P, K=100, N=50, st=None), **k}.values())  # noqa: E731
     assert p(w=None) == -1 and p(p=None) == -1 and p(ldw=49) == -2 and p(p=P + 8) == -3 and p(N=0) == -2
     z = lambda **k: lib.souffle_int8_quantize_weight(*{**dict(w=P, t=0, ldw=50, p=P, s=P, K=100, N=50, st=None), **k}.values())  # noqa: E731
@@ -203,7 +203,7 @@ def test_linear_types_and_epilogues(dtype, act, M, K, N, ldx, ldy):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,K,N", [(1, 16384, 40), (1, 16385, 40), (2, 4100, 5000), (3, 5461, 20), (4, 4096, 4200), (5, 777, 4101), (8, 2048, 64), (9, 1820, 65), (16, 1024, 300), (16, 1025, 300)])
+@pytest.mark.parametrize("M,K,N", [(1, 16384, 40), (1, 16385, 40), (2, 4100, 5000), (3, 5461, 20), (4, 4096, 4200), (5, 777, 4101), (8, 2048, 64), (9, 1820, 65), (16, 1024, 300), (16, 1025, 300), (17, 1024, 300), (33, 1024, 4000), (40, 1025, 300), (300, 1017, 1000), (31, 8, 70), (47, 7, 70), (512, 1000, 2040), (513, 1000, 2040)])
 def test_linear_few_rows(dtype, M, K, N):
     """Around the size up to which the product's workgroups quantise the rows themselves, for every split of the waves."""
     announce("linear_int8 %s M=%d K=%d N=%d" % (dtype, M, K, N))
