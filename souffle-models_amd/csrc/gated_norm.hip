@@ -45,8 +45,7 @@ struct RowReduce {
   }
   // Two sums for one barrier.
   __device__ __forceinline__ void sum2(float &v0, float &v1) {
-    v0 = wave_sum_dpp(v0);
-    v1 = wave_sum_dpp(v1);
+    wave_sum2_dpp(v0, v1);
     if constexpr (kWaves > 1) {
       float *r = reinterpret_cast<float *>(red) + turn * 2 * kWaves;
       turn ^= 1;
@@ -235,33 +234,41 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   typedef typename Vec8<T>::type V;
   constexpr int kSlots = WG / TPR;
   __shared__ __attribute__((aligned(16))) unsigned lds_red[WG / 64 * 4];
-  __shared__ float lds_sum[kSlots > 1 ? TPR * NV * 8 : 1];
+  constexpr int kSlotCols = TPR * NV * 8;
+  __shared__ __attribute__((aligned(16))) float lds_sum[kSlots > 1 ? kVectors * kSlots * kSlotCols : 1];
   const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
   const float inv_n = 1.0f / (float)n;
   RowReduce<TPR> red{lds_red + slot * 4 * RowReduce<TPR>::kWaves, 0};
 
   float sums[kVectors][NV][8] = {};
-  // The slots' sums of vector v, added in the slots' order, to out[0 .. cols) by the first slot.
-  auto collect = [&](int v, auto store) {
-    if constexpr (kSlots > 1) {
-      for (int s = 1; s < kSlots; ++s) {
-        if (slot == s)
+  // The sums of the vectors in `mask`, over the slots in their order: whole(v, c, eight of them) or one(v, c, sum).
+  auto collect = [&](int mask, auto whole, auto one) {
+    if constexpr (kSlots == 1) {
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v)
+        if (mask >> v & 1)
+#pragma unroll
+          for (int i = 0; i < NV; ++i) whole(v, c0 + i * TPR * 8, sums[v][i]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v)
+        if (mask >> v & 1)
 #pragma unroll
           for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) lds_sum[(i * 8 + e) * TPR + t] = sums[v][i][e];
-        __syncthreads();
-        if (slot == 0)
+            for (int e = 0; e < 8; ++e) lds_sum[(v * kSlots + slot) * kSlotCols + c0 + i * TPR * 8 + e] = sums[v][i][e];
+      __syncthreads();
+#pragma unroll 1
+      for (int v = 0; v < kVectors; ++v)
+        if (mask >> v & 1)
+          for (int c = threadIdx.x; c < n; c += WG) {
+            float s = 0.f;
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sums[v][i][e] += lds_sum[(i * 8 + e) * TPR + t];
-        __syncthreads();
-      }
+            for (int k = 0; k < kSlots; ++k) s += lds_sum[(v * kSlots + k) * kSlotCols + c];
+            one(v, c, s);
+          }
+      __syncthreads();
     }
-    if (slot == 0)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) store(c0 + i * TPR * 8, sums[v][i]);
   };
 
   // a gradient that is not there: x instead, taken as zeros
@@ -401,7 +408,8 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
       for (int i = 0; i < NV; ++i) store_row<FORM>(static_cast<T *>(a.df) + row * a.ld_df, c0 + i * TPR * 8, a.df && valid ? n : 0, from_f32<T>(d[i]));
     }
     if (a.dgate && a.chunks_per_gate == 0) {      // the gate row's rows were all this workgroup's
-      collect(kGate, [&](int c, const float (&v)[8]) { store_row<FORM>(static_cast<T *>(a.dgate) + (long long)gr * n, c, n, from_f32<T>(v)); });
+      T *dg = static_cast<T *>(a.dgate) + (long long)gr * n;
+      collect(1 << kGate, [&](int, int c, const float (&s)[8]) { store_row<FORM>(dg, c, n, from_f32<T>(s)); }, [&](int, int c, float s) { dg[c] = (T)s; });
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -410,12 +418,8 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
     run = run_end;
   }
   float *out = a.partial + (long long)blockIdx.x * a.vectors * n;
-#pragma unroll
-  for (int v = 0; v < kVectors; ++v)
-    if (a.wanted >> v & 1) {
-      float *o = out + (long long)__popc(a.wanted & ((1 << v) - 1)) * n;
-      collect(v, [&](int c, const float (&s)[8]) { store_row<FORM>(o, c, n, from_f32<float>(s)); });
-    }
+  auto at = [&](int v) { return out + (long long)__popc(a.wanted & ((1 << v) - 1)) * n; };
+  collect(a.wanted, [&](int v, int c, const float (&s)[8]) { store_row<FORM>(at(v), c, n, from_f32<float>(s)); }, [&](int v, int c, float s) { at(v)[c] = s; });
 }
 
 struct FinishArgs {
@@ -423,11 +427,12 @@ struct FinishArgs {
   void *out[kVectors];
   int cols, vectors, wanted, chunks, chunks_per_gate;
 };
-// Column sums over the chunks: 64 columns x 16 slices of the chunks per workgroup, slices added in order.
+// Column sums over the chunks: 32 columns x 32 slices of the chunks per workgroup, slices added in order.  With 256 chunks a thread has
+// eight loads, all under way at once.
 template <class T>
 __global__ void __launch_bounds__(1024) k_gated_norm_grad_finish(const FinishArgs a) {
-  __shared__ float lds[16][64];
-  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  __shared__ float lds[32][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   int v = 0, seen = 0, first = 0, count = a.chunks;
   long long row = 0;
   // blockIdx.y: the wanted vectors in order, then the gate's further rows
@@ -448,15 +453,15 @@ __global__ void __launch_bounds__(1024) k_gated_norm_grad_finish(const FinishArg
   float s = 0.f;
   if (c < a.cols) {
     const float *p = a.partial + ((long long)first * a.vectors + y) * a.cols + c;
-#pragma unroll 4
-    for (int k = slice; k < count; k += 16) s += p[(long long)k * a.vectors * a.cols];
+#pragma unroll 8
+    for (int k = slice; k < count; k += 32) s += p[(long long)k * a.vectors * a.cols];
   }
   lds[slice][lane] = s;
   __syncthreads();
   if (slice == 0 && c < a.cols) {
     s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += lds[k][lane];
+    for (int k = 0; k < 32; ++k) s += lds[k][lane];
     static_cast<T *>(a.out[v])[row * a.cols + c] = (T)s;
   }
 }
@@ -583,7 +588,7 @@ static int backward(const BwdArgs &a, const FinishArgs &f, int gate_rows, hipStr
                             : a.cols % 8 ? rows_backward<kRagged, T>(a, f.chunks, st) : rows_backward<kWhole, T>(a, f.chunks, st);
   if (rc || f.vectors == 0) return rc;
   const int more = (f.wanted >> kGate & 1) ? gate_rows - 1 : 0;
-  hipLaunchKernelGGL(k_gated_norm_grad_finish<T>, dim3((a.cols + 63) / 64, f.vectors + more), dim3(1024), 0, st, f);
+  hipLaunchKernelGGL(k_gated_norm_grad_finish<T>, dim3((a.cols + 31) / 32, f.vectors + more), dim3(1024), 0, st, f);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }

@@ -128,6 +128,18 @@ __device__ __forceinline__ float wave_sum_dpp(float v) {
   v += dpp<0x143, 12>(v, 0.f);      // row_bcast:31 into rows 2 and 3
   return lane63(v);
 }
+// Two sums in one chain: after the halves of both change places, one half of the wave sums v0 and the other v1.
+__device__ __forceinline__ void wave_sum2_dpp(float &v0, float &v1) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v0), __builtin_bit_cast(unsigned, v1), false, false);
+  float v = __builtin_bit_cast(float, (unsigned)p[0]) + __builtin_bit_cast(float, (unsigned)p[1]);
+  v += dpp<0x111, 15>(v, 0.f);
+  v += dpp<0x112, 15>(v, 0.f);
+  v += dpp<0x114, 15>(v, 0.f);
+  v += dpp<0x118, 15>(v, 0.f);
+  v += dpp<0x142, 10>(v, 0.f);
+  v0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 31));
+  v1 = lane63(v);
+}
 // Largest of non-negative floats or NaNs, as bit patterns: NaN > infinity > finite, so a NaN is never lost.
 __device__ __forceinline__ unsigned wave_umax_dpp(unsigned v) {
 #define SOUFFLE_STEP(CTRL, ROWS) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 15, false))
