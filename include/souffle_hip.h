@@ -394,11 +394,12 @@ enum { SOUFFLE_F16 = 0, SOUFFLE_BF16 = 1, SOUFFLE_F32 = 2 };
 
 /* ------------------------------------------------- 8-bit linear layers ---- */
 /* y = act(s[m] t[n] sum_k q[m][k] w[k][n] + bias[n]): rows in 8-bit integers with one scale per row, weights with one per
- * output channel; the sums are exact 32-bit integers.  K <= 131071.
+ * output channel; the sums are exact 32-bit integers.  K <= 131071, M <= 2^30.
  * A row x becomes q = round_half_even(x / s) with s = max(fp32(max |x| / 127), 2^-100): the rounding of the real quotient.
  * A row that holds a NaN or an infinity gets s = NaN (and q = 0), so that all results computed from it are NaN.
  * q lies in rows of ldq bytes, ldq a multiple of 16 and at least K rounded up to 64; the bytes behind K are multiplied
  * by zeros, whatever they hold.
+ * No output overlaps an input.
  * Weights are kept packed (souffle_int8_packed_bytes = K and N rounded up to 64, multiplied; 16-byte aligned), made once
  * when a model is loaded: the bytes of weight (k, n) lie at
  *     ((n / 64 * ceil(K / 64) + k / 64) * 4 + n / 4 % 4) * 1024 + (k / 16 % 4 * 16 + n / 16 % 4 * 4 + n % 4) * 16 + k % 16
@@ -426,7 +427,7 @@ int souffle_linear_int8(const void *x, long long ldx, const void *packed, const 
  * absent (NONE).  With post_norm NONE, no gate and residual_scale 1, h is a post-norm encoder's LN(x + f). */
 enum { SOUFFLE_NORM_NONE = 0, SOUFFLE_NORM_LAYER = 1, SOUFFLE_NORM_RMS = 2 };
 typedef struct {
-  int rows, cols;                /* cols <= 16384 */
+  int rows, cols;                /* rows <= 2^30, cols <= 16384 */
   int dtype;                     /* SOUFFLE_F16 / BF16 / F32: of the rows and of all vectors */
   int post_norm, pre_norm;       /* SOUFFLE_NORM_*; pre_norm is LAYER or RMS */
   int rows_per_gate;             /* consecutive rows that share one row of gate (a sequence); 0: all rows share one */

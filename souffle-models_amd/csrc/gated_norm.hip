@@ -471,7 +471,7 @@ constexpr int kMaxCols = 16384;
 
 static int check_cfg(const souffle_gated_norm_cfg *c) {
   if (!c) return fail(SOUFFLE_ERR_NULL, "cfg is NULL");
-  if (c->rows < 0) return fail(SOUFFLE_ERR_SHAPE, "rows must not be negative (got %d)", c->rows);
+  if (c->rows < 0 || c->rows > (1 << 30)) return fail(SOUFFLE_ERR_SHAPE, "rows must be in 0..2^30 (got %d)", c->rows);
   if (c->cols < 1 || c->cols > kMaxCols) return fail(SOUFFLE_ERR_SHAPE, "cols must be in 1..%d (got %d)", kMaxCols, c->cols);
   if (c->dtype != SOUFFLE_F16 && c->dtype != SOUFFLE_BF16 && c->dtype != SOUFFLE_F32) return fail(SOUFFLE_ERR_SHAPE, "unknown dtype %d", c->dtype);
   if (c->post_norm < SOUFFLE_NORM_NONE || c->post_norm > SOUFFLE_NORM_RMS) return fail(SOUFFLE_ERR_SHAPE, "unknown post_norm %d", c->post_norm);
@@ -664,7 +664,7 @@ extern "C" int souffle_gated_norm_backward(const souffle_gated_norm_cfg *c, cons
   const void *vec[5] = {g->pre_gamma, g->pre_beta, g->gate, g->post_gamma, g->post_beta};
   for (const void *p : vec)
     if (reinterpret_cast<uintptr_t>(p) % (c->dtype == SOUFFLE_F32 ? 4 : 2)) return fail(SOUFFLE_ERR_ALIGN, "a gradient vector is not aligned to its elements");
-  const int rpg = c->rows_per_gate ? c->rows_per_gate : c->rows, wanted = wanted_vectors(g);
+  const int rpg = w->gate && c->rows_per_gate ? c->rows_per_gate : c->rows, wanted = wanted_vectors(g);
   if (wanted) {
     if (!ws || ws_bytes < souffle_gated_norm_backward_workspace_bytes(c))
       return fail(SOUFFLE_ERR_WORKSPACE, "workspace too small: need %zu bytes", souffle_gated_norm_backward_workspace_bytes(c));

@@ -13,7 +13,6 @@
 // results are the columns 16 g + 4 t .. + 3 of one row (g = lane / 16), so over the four operands a lane owns 16 adjacent columns of a row: 32
 // bytes of an fp16 result.
 #include <algorithm>
-#include <atomic>
 #include "typed.hpp"
 #include "host_util.hpp"
 
@@ -42,55 +41,57 @@ __device__ __forceinline__ i4 ldg16(const int8_t *p) { return *(const __attribut
 template <class T, int TPR, int NV, RowForm FORM>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T *x, long long ldx, int8_t *q, long long ldq, float *scale, int rows, int cols) {
   constexpr int kSlots = 256 / TPR;
-  __shared__ unsigned lds_max[4];
+  __shared__ unsigned lds_max[2][4];
   const int slot = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  const long long row = (long long)blockIdx.x * kSlots + slot;
-  if (TPR == 64 && row >= rows) return;      // (whole waves; with 256 threads per row every workgroup has a row)
-  const T *xr = x + row * ldx;
-  int8_t *qr = q + row * ldq;
-  typename Vec8<T>::type v[NV ? NV : 1];
-  unsigned m = 0u;
-  auto widen = [&](float (&f)[8], typename Vec8<T>::type w, int c) { to_f32(f, settle_row<FORM, T>(w, c, cols)); };
-  auto largest = [&](const float (&f)[8]) {
+  int turn = 0;      // (rows of 256 threads: every thread takes the same turns)
+  for (long long row = (long long)blockIdx.x * kSlots + slot; row < rows; row += (long long)gridDim.x * kSlots, turn ^= 1) {
+    const T *xr = x + row * ldx;
+    int8_t *qr = q + row * ldq;
+    typename Vec8<T>::type v[NV ? NV : 1];
+    unsigned m = 0u;
+    auto widen = [&](float (&f)[8], typename Vec8<T>::type w, int c) { to_f32(f, settle_row<FORM, T>(w, c, cols)); };
+    auto largest = [&](const float (&f)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
-  };
-  float f[NV ? NV : 1][8];
-  if constexpr (NV > 0) {
+      for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
+    };
+    float f[NV ? NV : 1][8];
+    if constexpr (NV > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = load_row<FORM>(xr, (i * TPR + t) * 8, cols);
+      for (int i = 0; i < NV; ++i) v[i] = load_row<FORM>(xr, (i * TPR + t) * 8, cols);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      widen(f[i], v[i], (i * TPR + t) * 8);
-      largest(f[i]);
+      for (int i = 0; i < NV; ++i) {
+        widen(f[i], v[i], (i * TPR + t) * 8);
+        largest(f[i]);
+      }
+    } else {
+      for (int c = t * 8; c < cols; c += TPR * 8) {
+        widen(f[0], load_row<FORM>(xr, c, cols), c);
+        largest(f[0]);
+      }
     }
-  } else {
-    for (int c = t * 8; c < cols; c += TPR * 8) {
-      widen(f[0], load_row<FORM>(xr, c, cols), c);
-      largest(f[0]);
+    m = wave_umax_dpp(m);
+    if constexpr (TPR > 64) {
+      unsigned *r = lds_max[turn];
+      if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = m;
+      __syncthreads();
+      m = max(max(r[0], r[1]), max(r[2], r[3]));
     }
+    const RowScale rs = row_scale(m);
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + t) * 8;
+        const u2 p = quantize8(f[i], rs);
+        if (c < cols) *reinterpret_cast<u2 *>(qr + c) = p;
+      }
+    } else {
+      for (int c = t * 8; c < cols; c += TPR * 8) {
+        widen(f[0], load_row<FORM>(xr, c, cols), c);
+        *reinterpret_cast<u2 *>(qr + c) = quantize8(f[0], rs);
+      }
+    }
+    if (t == 0) scale[row] = rs.scale;
   }
-  m = wave_umax_dpp(m);
-  if constexpr (TPR > 64) {
-    if ((threadIdx.x & 63) == 0) lds_max[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = max(max(lds_max[0], lds_max[1]), max(lds_max[2], lds_max[3]));
-  }
-  const RowScale rs = row_scale(m);
-  if constexpr (NV > 0) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * 8;
-      const u2 p = quantize8(f[i], rs);
-      if (c < cols) *reinterpret_cast<u2 *>(qr + c) = p;
-    }
-  } else {
-    for (int c = t * 8; c < cols; c += TPR * 8) {
-      widen(f[0], load_row<FORM>(xr, c, cols), c);
-      *reinterpret_cast<u2 *>(qr + c) = quantize8(f[0], rs);
-    }
-  }
-  if (t == 0) scale[row] = rs.scale;
 }
 
 // Byte offset of weight (k, n) in the packed copy.
@@ -390,7 +391,7 @@ template <class T, int MI, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
   constexpr int kWaves = WM * WN, kBM = 16 * MI * WM, kStage = kBM * 128, kLoads = kBM / 8 / kWaves, kWLoads = 8;
   static_assert(kLoads * kWaves * 8 == kBM, "every wave fills the same number of KB of a stage");
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[3 * kStage + (kBM + 64 * WN) * 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   // Workgroup b runs on XCD b % 8: each XCD takes a run of tiles, eight rows of tiles deep, so that what its L2 holds is shared.
   const int row_tiles = (a.M + kBM - 1) / kBM, tiles = row_tiles * a.col_tiles;
@@ -520,6 +521,7 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
 
 // ------------------------------------------------------------------------------------------- host side ----
 constexpr int kMaxK = 131071;      // 128 * 128 * K stays below 2^31
+constexpr int kMaxRows = 1 << 30;
 
 static bool known_dtype(int t) { return t == SOUFFLE_F16 || t == SOUFFLE_BF16 || t == SOUFFLE_F32; }
 static unsigned size_of(int t) { return t == SOUFFLE_F32 ? 4 : 2; }
@@ -540,9 +542,10 @@ static int check_x(const char *name, const void *x, int dtype, long long ld, int
   return SOUFFLE_OK;
 }
 
+constexpr int kMostRowGroups = 1 << 22;      // (a launch holds fewer than 2^32 threads; beyond that a workgroup takes several rows)
 template <RowForm FORM, class T>
 static void launch_quantize(const T *x, long long ldx, int8_t *q, long long ldq, float *scale, int M, int K, hipStream_t st) {
-  const dim3 wide(M), narrow((M + 3) / 4), block(256);
+  const dim3 wide(std::min(M, kMostRowGroups)), narrow(std::min((M + 3) / 4, kMostRowGroups)), block(256);
   if (K <= 512) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1, FORM>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
   else if (K <= 1024) hipLaunchKernelGGL((k_quantize_rows<T, 64, 2, FORM>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
   else if (K <= 2048) hipLaunchKernelGGL((k_quantize_rows<T, 256, 1, FORM>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
@@ -553,7 +556,7 @@ static void launch_quantize(const T *x, long long ldx, int8_t *q, long long ldq,
 template <class T>
 static int quantize_rows(const void *xv, long long ldx, int8_t *q, long long ldq, float *scale, int M, int K, hipStream_t st) {
   const T *x = static_cast<const T *>(xv);
-  if (K < 8) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1, kShort>), dim3((M + 3) / 4), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K);
+  if (K < 8) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1, kShort>), dim3(std::min((M + 3) / 4, kMostRowGroups)), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K);
   else if (K % 8) launch_quantize<kRagged>(x, ldx, q, ldq, scale, M, K, st);
   else launch_quantize<kWhole>(x, ldx, q, ldq, scale, M, K, st);
   SOUFFLE_HIP_TRY(hipGetLastError());
@@ -566,26 +569,17 @@ static int quantize_rows(const void *x, int dtype, long long ldx, int8_t *q, lon
 }
 
 // One workgroup per tile.  (Tiles narrower than 64 columns interleave: there are 64 / cols of them for any part of 64.)
-static int grid_of(const Args &a, int rows, int cols, unsigned *grid, int *col_tiles) {
+static int grid_of(const Args &a, int rows, int cols, int threads, unsigned *grid, int *col_tiles) {
   *col_tiles = cols < 64 ? (a.N + 63) / 64 * (64 / cols) : (a.N + cols - 1) / cols;
   const long long n = (long long)*col_tiles * ((a.M + rows - 1) / rows);
-  if (n > 0x7fffffff) return fail(SOUFFLE_ERR_SHAPE, "M = %d rows of N = %d are more tiles than one launch holds", a.M, a.N);
+  if (n * threads > 0xffffffffll) return fail(SOUFFLE_ERR_SHAPE, "M = %d rows of N = %d are more tiles than one launch holds", a.M, a.N);
   *grid = (unsigned)n;
-  return SOUFFLE_OK;
-}
-// The kernel may use `bytes` of LDS on the current device (set once per device and kernel).
-static int allow_lds(const void *kernel, int bytes, std::atomic<unsigned> &done) {
-  int dev = 0;
-  SOUFFLE_HIP_TRY(hipGetDevice(&dev));
-  if (done.load() >> dev & 1) return SOUFFLE_OK;
-  SOUFFLE_HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.fetch_or(1u << dev);
   return SOUFFLE_OK;
 }
 template <class T, int MF, int NF, int W, int U>
 static int launch_split(Args a, hipStream_t st) {
   unsigned grid;
-  if (int rc = grid_of(a, 16 * MF, 16 * NF, &grid, &a.col_tiles)) return rc;
+  if (int rc = grid_of(a, 16 * MF, 16 * NF, W * 64, &grid, &a.col_tiles)) return rc;
   hipLaunchKernelGGL((k_gemm_split<T, MF, NF, W, U, false>), dim3(grid), dim3(W * 64), 0, st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
@@ -593,19 +587,16 @@ static int launch_split(Args a, hipStream_t st) {
 template <class T, int NF, int U>
 static int launch_rows(Args a, hipStream_t st) {
   unsigned grid;
-  if (int rc = grid_of(a, 16, 16 * NF, &grid, &a.col_tiles)) return rc;
+  if (int rc = grid_of(a, 16, 16 * NF, 512, &grid, &a.col_tiles)) return rc;
   hipLaunchKernelGGL((k_gemm_split<T, 1, NF, 8, U, true>), dim3(grid), dim3(512), a.M * (a.kblocks * 64 + 16), st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
 template <class T, int MI, int WM, int WN>
 static int launch_tile(Args a, hipStream_t st) {
-  constexpr int kBM = 16 * MI * WM, kLds = 3 * kBM * 128 + (kBM + 64 * WN) * 4;
-  static std::atomic<unsigned> done{0};
-  if (int rc = allow_lds((const void *)k_gemm_tile<T, MI, WM, WN>, kLds, done)) return rc;
   unsigned grid;
-  if (int rc = grid_of(a, kBM, 64 * WN, &grid, &a.col_tiles)) return rc;
-  hipLaunchKernelGGL((k_gemm_tile<T, MI, WM, WN>), dim3(grid), dim3(WM * WN * 64), kLds, st, a);
+  if (int rc = grid_of(a, 16 * MI * WM, 64 * WN, WM * WN * 64, &grid, &a.col_tiles)) return rc;
+  hipLaunchKernelGGL((k_gemm_tile<T, MI, WM, WN>), dim3(grid), dim3(WM * WN * 64), 0, st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
@@ -645,7 +636,7 @@ static int linear_rows(const Args &a, hipStream_t st) {
 
 static int check_product(const void *packed, const float *col_scale, const void *bias, int act, const void *y, int dtype, long long ldy, int M,
                          int N, int K) {
-  if (M < 0) return fail(SOUFFLE_ERR_SHAPE, "M must not be negative (got %d)", M);
+  if (M < 0 || M > kMaxRows) return fail(SOUFFLE_ERR_SHAPE, "M must be in 0..2^30 (got %d)", M);
   if (int rc = check_kn(K, N)) return rc;
   if (!known_dtype(dtype)) return fail(SOUFFLE_ERR_SHAPE, "unknown dtype %d", dtype);
   if (act != SOUFFLE_ACT_NONE && act != SOUFFLE_ACT_RELU && act != SOUFFLE_ACT_GELU_TANH && act != SOUFFLE_ACT_GELU_ERF)
@@ -702,7 +693,7 @@ extern "C" int souffle_int8_quantize_weight(const void *w, int dtype, long long 
 
 extern "C" int souffle_quantize_rows(const void *x, int dtype, long long ldx, int8_t *q, long long ldq, float *row_scale, int M, int K,
                                      souffle_stream_t stream) {
-  if (M < 0) return fail(SOUFFLE_ERR_SHAPE, "M must not be negative (got %d)", M);
+  if (M < 0 || M > kMaxRows) return fail(SOUFFLE_ERR_SHAPE, "M must be in 0..2^30 (got %d)", M);
   if (int rc = check_kn(K, 1)) return rc;
   if (!known_dtype(dtype)) return fail(SOUFFLE_ERR_SHAPE, "unknown dtype %d", dtype);
   if (M == 0) return SOUFFLE_OK;
@@ -729,7 +720,7 @@ extern "C" int souffle_gemm_int8(const int8_t *q, long long ldq, const float *ro
 }
 
 extern "C" size_t souffle_linear_int8_workspace_bytes(int M, int N, int K) {
-  if (M < 0 || check_kn(K, N) || rows_in_kernel(M, K)) return 0;
+  if (M < 0 || M > kMaxRows || check_kn(K, N) || rows_in_kernel(M, K)) return 0;
   return round_up((size_t)M * round_up(K, 64) + (size_t)M * 4, 256);
 }
 

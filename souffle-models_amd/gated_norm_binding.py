@@ -12,7 +12,8 @@ of all three:
     gate                    [D], or [G, D]: one row for each of G equal runs of rows (a sequence), or None
     residual_scale, post_eps, pre_eps               numbers
 Statistics and sums are in fp32, h comes from y before y is rounded, and two calls give the same bits.  Work is queued on
-the current stream of the tensors' device and nothing is kept between calls.
+the current stream of the tensors' device and nothing is kept between calls.  Autograd does not record these calls:
+a training step calls gated_norm_backward (or an autograd function around the two does).
 """
 import ctypes as C
 import functools

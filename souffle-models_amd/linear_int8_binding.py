@@ -8,6 +8,7 @@
 A row x is held as q = round_half_even(x / s), s = max(max|x| / 127, 2^-100) in fp32, a weight column likewise; products
 sum in exact 32-bit integers.  A row with a NaN or an infinity gives a row of NaN.  Work is queued on the current
 stream of the tensors' device; nothing is kept between calls, so calls may overlap on several streams and be captured.
+Autograd does not record these calls.
 """
 from typing import NamedTuple
 
@@ -84,6 +85,16 @@ def _output(out, like, rows, n, dtype, index):
     if out.dtype != dtype or tuple(out.shape) != (rows, n):
         raise ValueError("out must be [%d, %d] of %s" % (rows, n, dtype))
     return _rows("out", out)
+
+
+def _check_apart(x, ldx, out, ldy):
+    """The rows of x and of out, both of one type, have no element in common (some are still read when others are written)."""
+    size, a, b = x.element_size(), x.data_ptr(), out.data_ptr()
+    if not x.numel() or a + ((x.shape[0] - 1) * ldx + x.shape[1]) * size <= b or b + ((out.shape[0] - 1) * ldy + out.shape[1]) * size <= a:
+        return
+    gap = (b - a) % (ldx * size)
+    if ldx != ldy or gap < x.shape[1] * size or gap + out.shape[1] * size > ldx * size:      # (else: columns side by side in one buffer)
+        raise ValueError("out must not overlap x")
 
 
 def pack_weight(weight_q, scale):
@@ -165,7 +176,7 @@ def gemm_int8(q, row_scale, weight, *, bias=None, act=None, dtype=torch.float16,
 
 def linear_int8(x, weight, *, bias=None, act=None, out=None):
     """act(x . W + bias) with the rows of x [..., K] in 8 bits: quantize_rows and gemm_int8 in one call, bit for bit.
-    Returns [rows, N] of x's type; bias is of that type too."""
+    Returns [rows, N] of x's type; bias is of that type too.  out must not overlap x."""
     index = _check_cuda("x", x)
     if not sh.is_current(index):
         with torch.cuda.device(index):
@@ -178,7 +189,10 @@ def linear_int8(x, weight, *, bias=None, act=None, out=None):
     if x.shape[1] != K:
         raise ValueError("x must be [..., %d]" % K)
     b, a = _epilogue(bias, act, N, x.dtype, index)
+    given = out is not None
     out, ldy = _output(out, x, M, N, x.dtype, index)
+    if given:
+        _check_apart(x, ld, out, ldy)
     lib = sh.lib()
     nbytes = lib.souffle_linear_int8_workspace_bytes(M, N, K)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None

@@ -274,6 +274,23 @@ def test_empty_and_leading_dimensions():
 
 
 @gpu
+def test_out_beside_x_in_one_buffer_and_never_over_it():
+    announce("linear_int8: out and x in one buffer")
+    import linear_int8_binding as lb
+    for M in (3, 200):
+        w = lb.quantize_weight(values(3, 64, 48).cuda())
+        buf = values(4, M, 128, dtype=torch.float16).cuda()
+        y = lb.linear_int8(buf[:, :64].contiguous(), w)
+        for bad in (buf[:, :48], buf[:, 63:111], buf.view(-1)[64 * M:64 * M + 48 * M].view(M, 48)):
+            with pytest.raises(ValueError, match="overlap"):
+                lb.linear_int8(buf[:, :64], w, out=bad)
+        assert lb.linear_int8(buf[:, :64], w, out=buf[:, 80:]) is not None
+        assert torch.equal(buf[:, 80:], y)
+        big = values(5, 2 * M, 64, dtype=torch.float16).cuda()
+        assert torch.equal(lb.linear_int8(big[M:], w, out=big[:M, :48]), lb.linear_int8(big[M:], w))
+
+
+@gpu
 def test_rows_beyond_two_gib():
     """Offsets of a long activation pass 31 bits: rows 70000 apart by 32800 elements."""
     announce("linear_int8: offsets beyond 2^31")
