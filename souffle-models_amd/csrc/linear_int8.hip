@@ -390,7 +390,7 @@ __device__ const int8_t zero_bytes[16] __attribute__((aligned(16))) = {};
 template <class T, int MI, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
   constexpr int kWaves = WM * WN, kBM = 16 * MI * WM, kStage = kBM * 128, kLoads = kBM / 8 / kWaves, kWLoads = 8;
-  static_assert(kLoads * kWaves * 8 == kBM, "every wave fills the same number of KB of a stage");
+  static_assert(kLoads * kWaves * 8 == kBM && kLoads <= MI && kWLoads % MI == 0, "every wave fills the same number of KB of a stage, in half a step");
   __shared__ __attribute__((aligned(16))) unsigned char lds[3 * kStage + (kBM + 64 * WN) * 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   // Workgroup b runs on XCD b % 8: each XCD takes a run of tiles, eight rows of tiles deep, so that what its L2 holds is shared.
@@ -411,22 +411,12 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
     chunk[i] = ((lane & 7) ^ (row >> 1 & 7)) * 16;
   }
   // (behind K's end: zeros, so that steps come in pairs, always with the same loads, and the loop has no branch)
-  auto stage_in = [&](int s, int slot) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int off = s * 128 + chunk[i];
-      load_lds16(off < k_end ? src[i] + off : zero_bytes, lds0 + slot * kStage + (wave * kLoads + i) * 1024);
-    }
+  auto stage_in = [&](int s, int slot, int i) {
+    const int off = s * 128 + chunk[i];
+    load_lds16(off < k_end ? src[i] + off : zero_bytes, lds0 + slot * kStage + (wave * kLoads + i) * 1024);
   };
   const int8_t *wp = a.packed + (size_t)min(group, last_group) * a.kblocks * 4096 + lane * 16;
-  auto fetch_w = [&](i4 (&w)[2][4], int s) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int8_t *p = wp + (size_t)min(2 * s + h, a.kblocks - 1) * 4096;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[h][j] = ldg16(p + j * 1024);
-    }
-  };
+  auto fetch_w = [&](i4 (&w)[2][4], int s, int i) { w[i / 4][i % 4] = ldg16(wp + (size_t)min(2 * s + i / 4, a.kblocks - 1) * 4096 + i % 4 * 1024); };
   i4 acc[MI][4];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -439,17 +429,19 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
   };
   // Stage s of the ring with its weights in w; those of s + 1 go to wnext.  The 2 MI operands of rows are read two ahead of their use, across
   // the step's end, so the one barrier of a step stands in its middle: it says that the rows of s + 1 are there and that nobody reads
-  // those of s - 1 any more.  A wave's loads are queued in the order weights of s + 1, rows of s + 2 | ...  The
+  // those of s - 1 any more.  A wave's loads are queued one by one between the matrix instructions (in a burst, all waves at once, each
+  // stands still until the texture unit takes its next one), in the order weights of s + 1, rows of s + 2 | ...  The
   // compiler waits for weights at their first use and does not count the direct loads, so these are queued behind
   // the step's last first use: its count, too small by that many, then only asks for loads that are a step old.
   i4 x0, x1;
   auto step = [&](int s, int slot, i4 (&w)[2][4], i4 (&wnext)[2][4]) {
     const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
-    fetch_w(wnext, s + 1);
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < 2 * MI; ++u) {
       const i4 x2 = u + 2 < 2 * MI ? row16(slot, (u + 2) % MI, (u + 2) / MI) : row16(slot1, u + 2 - 2 * MI, 0);
+      if (u < MI)
+#pragma unroll
+        for (int i = u * kWLoads / MI; i < (u + 1) * kWLoads / MI; ++i) fetch_w(wnext, s + 1, i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[u % MI][j] = mfma_i8(w[u / MI][j], x0, acc[u % MI][j]);
       x0 = x1;
@@ -460,7 +452,7 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
         compiler_fence();
       }
       __builtin_amdgcn_sched_barrier(0);      // (otherwise the reads sink to their uses)
-      if (u == MI) stage_in(s + 2, slot2);
+      if (u >= MI && u - MI < kLoads) stage_in(s + 2, slot2, u - MI);
     }
   };
   // The scales of the tile's rows and columns wait for the epilogue in LDS, behind the stages.
@@ -472,9 +464,12 @@ __global__ void __launch_bounds__(WM * WN * 64) k_gemm_tile(const Args a) {
     if (part < kBM / 64 + WN) load_lds4(from, lds0 + 3 * kStage + part * 256);
   }
   i4 w0[2][4], w1[2][4];
-  stage_in(0, 0);
-  stage_in(1, 1);
-  fetch_w(w0, 0);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) stage_in(0, 0, i);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) stage_in(1, 1, i);
+#pragma unroll
+  for (int i = 0; i < kWLoads; ++i) fetch_w(w0, 0, i);
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWLoads + kLoads) : "memory");
   __builtin_amdgcn_s_barrier();
   compiler_fence();
