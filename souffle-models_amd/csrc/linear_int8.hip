@@ -173,20 +173,27 @@ __device__ __forceinline__ void with_activation(int act, F f) {
   else f(ActTag<SOUFFLE_ACT_GELU_ERF>());
 }
 
-// Columns n .. n+3 of row m.
+// Scales and bias of four columns from n.
+template <class T>
+struct Columns4 {
+  float scale[4], bias[4];
+  __device__ __forceinline__ void load(const Args &a, int n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = min(n + e, a.N - 1);
+      scale[e] = a.col_scale[c];
+      bias[e] = a.bias ? (float)static_cast<const T *>(a.bias)[c] : 0.f;
+    }
+  }
+};
 template <class T, int ACT>
-__device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s, float rs) {
+__device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s, float rs, const Columns4<T> &col) {
   T *y = static_cast<T *>(a.y) + m * a.ldy + n;
-  const T *bias = static_cast<const T *>(a.bias);
   typedef T V4 __attribute__((ext_vector_type(4)));
   typedef T V4u __attribute__((ext_vector_type(4), aligned(sizeof(T))));
   V4 out;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int c = min(n + e, a.N - 1);
-    const float v = ((float)s[e] * a.col_scale[c]) * rs + (bias ? (float)bias[c] : 0.f);
-    out[e] = (T)activate<ACT>(v);
-  }
+  for (int e = 0; e < 4; ++e) out[e] = (T)activate<ACT>(((float)s[e] * col.scale[e]) * rs + col.bias[e]);
   if (n + 4 <= a.N) {
     *reinterpret_cast<V4u *>(y) = out;
   } else {
@@ -208,6 +215,7 @@ template <class T, int MF, int NF, int W, int U, bool ROWS>
 __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
   static_assert(4 % NF == 0, "operands of the four that 64 columns have");
   static_assert(!ROWS || MF == 1, "rows of one operand");
+  static_assert(MF * NF <= W, "four results per thread");
   constexpr int kParts = 4 / NF;
   __shared__ i4 lds[W][MF * NF][64];
   __shared__ float lds_scale[16];
@@ -237,6 +245,15 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
     }
   };
   if (k_first < k_end) fetch(k_first);
+  // The thread's four results and what their epilogue needs, asked for now.
+  const int out_tile = threadIdx.x >> 6, out_m = m0 + 16 * (out_tile / NF) + (lane & 15), out_n = group * 64 + 16 * (lane >> 4) + 4 * (t0 + out_tile % NF);
+  const bool has_out = out_tile < MF * NF && out_m < a.M && out_n < a.N;
+  Columns4<T> columns;
+  float rs = 0.f;
+  if (has_out) {
+    columns.load(a, out_n);
+    if constexpr (!ROWS) rs = a.row_scale[out_m];
+  }
   if constexpr (ROWS) {
     // as many waves per row as there are for M rows at a time
     __shared__ unsigned lds_max[2][W];
@@ -303,15 +320,12 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
 #pragma unroll
     for (int j = 0; j < NF; ++j) lds[wave][i * NF + j][lane] = acc[i][j];
   __syncthreads();
-  with_activation(a.act, [&](auto act) {
-    for (int u = threadIdx.x; u < MF * NF * 64; u += W * 64) {
-      const int tile = u >> 6, l = u & 63, m = m0 + 16 * (tile / NF) + (l & 15), n = group * 64 + 16 * (l >> 4) + 4 * (t0 + tile % NF);
-      i4 s = lds[0][tile][l];
+  if (!has_out) return;
+  if constexpr (ROWS) rs = lds_scale[out_m];
+  i4 sum = lds[0][out_tile][lane];
 #pragma unroll
-      for (int w = 1; w < W; ++w) s += lds[w][tile][l];
-      if (m < a.M && n < a.N) finish4<T, decltype(act)::value>(a, m, n, s, ROWS ? lds_scale[m] : a.row_scale[m]);
-    }
-  });
+  for (int w = 1; w < W; ++w) sum += lds[w][out_tile][lane];
+  with_activation(a.act, [&](auto act) { finish4<T, decltype(act)::value>(a, out_m, out_n, sum, rs, columns); });
 }
 
 // Rows of 16 lanes: the odd ones of a change places with the even ones of b (permlane16), the upper two of a with the lower two of b (permlane32).
