@@ -73,13 +73,20 @@ struct RowReduce {
   }
 };
 
-// The vector's elements c .. c+7, or `missing` where the caller has none; zeros behind the row's end, which keep what is computed there zero.
+// A vector's elements c .. c+7, or `missing` where the caller has none; zeros behind the row's end, which keep what is computed
+// there zero.  In two steps, so that the loads of all vectors are under way before the first is waited for: a missing
+// vector's are made from `any`, a row of n, as a branch around them would wait at its end.
 template <RowForm FORM, class T>
-__device__ __forceinline__ typename Vec8<T>::type param8(const void *p, int c, int n, float missing) {
-  if (p) return settle_row<FORM, T>(load_row<FORM>(static_cast<const T *>(p), c, n), c, n);
-  typename Vec8<T>::type v;
+__device__ __forceinline__ typename Vec8<T>::type param_load(const void *p, const void *any, int c, int n) {
+  return load_row<FORM>(static_cast<const T *>(p ? p : any), c, n);
+}
+template <RowForm FORM, class T>
+__device__ __forceinline__ typename Vec8<T>::type param_settle(typename Vec8<T>::type v, const void *p, int c, int n, float missing) {
+  v = settle_row<FORM, T>(v, c, n);
+  if (!p) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (T)(c + e < n ? missing : 0.f);
+    for (int e = 0; e < 8; ++e) v[e] = (T)(c + e < n ? missing : 0.f);
+  }
   return v;
 }
 
@@ -129,18 +136,8 @@ __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
   const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
   RowReduce<TPR> red{lds_red + slot * 4 * RowReduce<TPR>::kWaves, 0};
 
-  V pg[NV], pb[NV], gt[NV], ng[NV], nb[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = c0 + i * TPR * 8;
-    pg[i] = param8<FORM, T>(a.post_gamma, c, n, 1.f);
-    pb[i] = param8<FORM, T>(a.post_beta, c, n, 0.f);
-    ng[i] = param8<FORM, T>(a.pre_gamma, c, n, 1.f);
-    nb[i] = param8<FORM, T>(a.pre_beta, c, n, 0.f);
-    gt[i] = param8<FORM, T>(nullptr, c, n, 1.f);
-  }
   const int first = (blockIdx.x * kSlots + slot) * a.rows_per_slot, end = min(first + a.rows_per_slot, a.rows);
-  int gate_row = -1;
+  if (TPR == 64 && first >= end) return;      // (rows of several waves: every workgroup has one)
   V xv[NV], fv[NV];
   auto fetch = [&](int row) {
     const T *x = static_cast<const T *>(a.x) + row * a.ldx, *f = static_cast<const T *>(a.f) + row * a.ldf;
@@ -150,15 +147,38 @@ __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
       fv[i] = load_row<FORM>(f, c0 + i * TPR * 8, n);
     }
   };
+  fetch(first);
+  int gate_row = first / a.rows_per_gate;
+  auto gate_at = [&](int row) { return a.gate ? static_cast<const T *>(a.gate) + (long long)row * n : nullptr; };
+  V pg[NV], pb[NV], gt[NV], ng[NV], nb[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = c0 + i * TPR * 8;
+    pg[i] = param_load<FORM, T>(a.post_gamma, a.x, c, n);
+    pb[i] = param_load<FORM, T>(a.post_beta, a.x, c, n);
+    gt[i] = param_load<FORM, T>(gate_at(gate_row), a.x, c, n);
+    ng[i] = param_load<FORM, T>(a.pre_gamma, a.x, c, n);
+    nb[i] = param_load<FORM, T>(a.pre_beta, a.x, c, n);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = c0 + i * TPR * 8;
+    pg[i] = param_settle<FORM, T>(pg[i], a.post_gamma, c, n, 1.f);
+    pb[i] = param_settle<FORM, T>(pb[i], a.post_beta, c, n, 0.f);
+    gt[i] = param_settle<FORM, T>(gt[i], a.gate, c, n, 1.f);
+    ng[i] = param_settle<FORM, T>(ng[i], a.pre_gamma, c, n, 1.f);
+    nb[i] = param_settle<FORM, T>(nb[i], a.pre_beta, c, n, 0.f);
+  }
   // (rows of several waves: one row per workgroup at a time, so every thread takes the same turns through the barriers)
-  if (first < end) fetch(first);
   for (int row = first; row < end; ++row) {
     if (a.gate) {
       const int gr = row / a.rows_per_gate;
       if (gr != gate_row) {
         gate_row = gr;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) gt[i] = param8<FORM, T>(static_cast<const T *>(a.gate) + (long long)gr * n, c0 + i * TPR * 8, n, 1.f);
+        for (int i = 0; i < NV; ++i) gt[i] = param_load<FORM, T>(gate_at(gr), nullptr, c0 + i * TPR * 8, n);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) gt[i] = settle_row<FORM, T>(gt[i], c0 + i * TPR * 8, n);
       }
     }
     float x[NV][8], p[NV][8];
@@ -287,17 +307,15 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   for (int run = first; run < end;) {
     const int gr = run / a.rows_per_gate, run_end = min((gr + 1) * a.rows_per_gate, end);
     V gt[NV], pg[NV], pb[NV], ng[NV];
-    auto vectors = [&]() {
+    const void *gate = a.gate ? static_cast<const T *>(a.gate) + (long long)gr * n : nullptr;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = c0 + i * TPR * 8;
-        gt[i] = param8<FORM, T>(a.gate ? static_cast<const T *>(a.gate) + (long long)gr * n : nullptr, c, n, 1.f);
-        pg[i] = param8<FORM, T>(a.post_gamma, c, n, 1.f);
-        pb[i] = param8<FORM, T>(a.post_beta, c, n, 0.f);
-        ng[i] = param8<FORM, T>(a.pre_gamma, c, n, 1.f);
-      }
-    };
-    vectors();
+    for (int i = 0; i < NV; ++i) {
+      const int c = c0 + i * TPR * 8;
+      gt[i] = param_load<FORM, T>(gate, a.x, c, n);
+      pg[i] = param_load<FORM, T>(a.post_gamma, a.x, c, n);
+      pb[i] = param_load<FORM, T>(a.post_beta, a.x, c, n);
+      ng[i] = param_load<FORM, T>(a.pre_gamma, a.x, c, n);
+    }
     V xv[NV], fv[NV], yv[NV], hv[NV];
     auto fetch = [&](int row) {      // (a slot without a row takes the run's first one, with gradients of zero)
       const bool valid = row < run_end;
@@ -312,6 +330,14 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
       }
     };
     if constexpr (KEEP) fetch(run + slot);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = c0 + i * TPR * 8;
+      gt[i] = param_settle<FORM, T>(gt[i], gate, c, n, 1.f);
+      pg[i] = param_settle<FORM, T>(pg[i], a.post_gamma, c, n, 1.f);
+      pb[i] = param_settle<FORM, T>(pb[i], a.post_beta, c, n, 0.f);
+      ng[i] = param_settle<FORM, T>(ng[i], a.pre_gamma, c, n, 1.f);
+    }
     for (int base = run; base < run_end; base += kSlots) {
       const int row = base + slot;
       const bool valid = row < run_end;
