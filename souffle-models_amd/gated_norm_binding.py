@@ -21,7 +21,7 @@ import functools
 import torch
 
 import souffle_hip as sh
-from linear_int8_binding import _DTYPES, _check_cuda, _rows
+from linear_int8_binding import _DTYPES, _check_cuda, _device, _rows, _stream
 
 _NORMS = {None: sh.NORM_NONE, "layer": sh.NORM_LAYER, "rms": sh.NORM_RMS}
 
@@ -32,13 +32,19 @@ def _cfg(*fields):
     return sh.GatedNormCfg(*fields)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(M, D, per_gate):
+    """Of a gradient call; the kinds of the norms and the type do not matter."""
+    return sh.lib().souffle_gated_norm_backward_workspace_bytes(_cfg(M, D, sh.F32, sh.NORM_RMS, sh.NORM_RMS, per_gate, 1.0, 0.0, 0.0, D, D, D, D))
+
+
 def _on_device(position):
     """Runs a function with the device of its argument `x`, at that position, as the current one."""
     def decorate(fn):
         @functools.wraps(fn)
         def call(*args, **kw):
             x = args[position] if len(args) > position else kw.get("x")
-            if not isinstance(x, torch.Tensor) or not x.is_cuda or sh.is_current(x.get_device()):
+            if not isinstance(x, torch.Tensor) or not x.is_cuda or x.get_device() == _device():
                 return fn(*args, **kw)
             with torch.cuda.device(x.get_device()):
                 return fn(*args, **kw)
@@ -103,7 +109,7 @@ def gated_norm(x, f, *, gate=None, residual_scale=1.0, post_norm="layer", post_g
     xr, fr, index, cfg, w = _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_eps, pre_norm, pre_gamma, pre_beta, pre_eps)
     y = _like(x) if want_y else None
     h = _like(x)
-    sh.check(sh.lib().souffle_gated_norm_forward(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), h.data_ptr(), sh.stream_of(index)))
+    sh.check(sh.lib().souffle_gated_norm_forward(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), h.data_ptr(), _stream(index)))
     return y, h
 
 
@@ -119,7 +125,7 @@ def gated_norm_int8(x, f, *, gate=None, residual_scale=1.0, post_norm="layer", p
     q = x.new_empty((M, ldq), dtype=torch.int8)
     scale = x.new_empty(M, dtype=torch.float32)
     sh.check(sh.lib().souffle_gated_norm_forward_int8(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), q.data_ptr(), ldq, scale.data_ptr(),
-                                                      sh.stream_of(index)))
+                                                      _stream(index)))
     return y, (q if D == ldq else q[:, :D]), scale
 
 
@@ -143,19 +149,20 @@ def gated_norm_backward(dy, dh, x, f, *, gate=None, residual_scale=1.0, post_nor
             raise ValueError("%s must have x's shape and type" % name)
         d, ld = _rows(name, d)
         incoming.append((d.data_ptr(), ld))
-    given = [n for n, v in (("post_gamma", post_gamma), ("post_beta", post_beta), ("pre_gamma", pre_gamma), ("pre_beta", pre_beta)) if v is not None]
+    vector_gate = gate if gate is not None and gate.dim() == 1 else None
+    given = [n for n, v in (("gate", vector_gate), ("post_gamma", post_gamma), ("post_beta", post_beta), ("pre_gamma", pre_gamma), ("pre_beta", pre_beta))
+             if v is not None]
     vectors = x.new_empty((len(given), D)) if M else x.new_zeros((len(given), D))      # (one allocation: each takes as long as a check of all)
     g = {"x": _like(x), "f": _like(x), "gate": None, "post_gamma": None, "post_beta": None, "pre_gamma": None, "pre_beta": None}
     g.update(zip(given, vectors.unbind(0)))
-    if gate is not None:
+    if gate is not vector_gate:
         g["gate"] = gate.new_empty(gate.shape) if M else gate.new_zeros(gate.shape)
     if M == 0:
         return g
     (dy_ptr, ld_dy), (dh_ptr, ld_dh) = incoming
     grad = sh.GatedNormGrad(g["x"].data_ptr(), g["f"].data_ptr(), sh.ptr(g["pre_gamma"]), sh.ptr(g["pre_beta"]), sh.ptr(g["gate"]),
                             sh.ptr(g["post_gamma"]), sh.ptr(g["post_beta"]), ld_dy, ld_dh, D, D)
-    lib = sh.lib()
-    nbytes = lib.souffle_gated_norm_backward_workspace_bytes(cfg)
+    nbytes = _workspace_bytes(M, D, cfg.rows_per_gate)
     ws = x.new_empty(nbytes, dtype=torch.uint8)
-    sh.check(lib.souffle_gated_norm_backward(cfg, w, dy_ptr, dh_ptr, xr.data_ptr(), fr.data_ptr(), grad, ws.data_ptr(), nbytes, sh.stream_of(index)))
+    sh.check(sh.lib().souffle_gated_norm_backward(cfg, w, dy_ptr, dh_ptr, xr.data_ptr(), fr.data_ptr(), grad, ws.data_ptr(), nbytes, _stream(index)))
     return g

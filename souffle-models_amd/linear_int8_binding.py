@@ -10,11 +10,17 @@ sum in exact 32-bit integers.  A row with a NaN or an infinity gives a row of Na
 stream of the tensors' device; nothing is kept between calls, so calls may overlap on several streams and be captured.
 Autograd does not record these calls.
 """
+import functools
 from typing import NamedTuple
 
 import torch
 
 import souffle_hip as sh
+
+# Index of the current device, and hipStream_t of a device's current stream, without the objects that torch.cuda makes of them
+# (they take 1.3 and 2.8 us, a call of one row some 8).
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
 
 _DTYPES = {torch.float16: sh.F16, torch.bfloat16: sh.BF16, torch.float32: sh.F32}
 _ACTS = {None: sh.ACT_NONE, "relu": sh.ACT_RELU, "gelu": sh.ACT_GELU_ERF, "gelu_tanh": sh.ACT_GELU_TANH}
@@ -59,12 +65,17 @@ def _check_weight(w, index):
         raise TypeError("weight must be an Int8Weight (quantize_weight, pack_weight)")
     packed, scale, K, N = w
     _check_cuda("weight.packed", packed, index)
-    _check_cuda("weight.scale", scale, index)
-    if packed.dtype != torch.int8 or not packed.is_contiguous() or packed.numel() != -(-K // 64) * -(-N // 64) * 4096:
+    if packed.dtype is not torch.int8 or packed.numel() != -(-K // 64) * -(-N // 64) * 4096 or not packed.is_contiguous():
         raise ValueError("weight.packed must hold the packed [%d, %d] matrix as contiguous int8" % (K, N))
-    if scale.dtype != torch.float32 or not scale.is_contiguous() or scale.numel() != N:
+    _check_cuda("weight.scale", scale, index)
+    if scale.dtype is not torch.float32 or scale.numel() != N or not scale.is_contiguous():
         raise ValueError("weight.scale must hold %d contiguous float32" % N)
     return packed.data_ptr(), scale.data_ptr(), K, N
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(M, N, K):
+    return sh.lib().souffle_linear_int8_workspace_bytes(M, N, K)
 
 
 def _epilogue(bias, act, n, dtype, index):
@@ -108,7 +119,7 @@ def pack_weight(weight_q, scale):
         raise ValueError("scale must be [%d] float32" % N)
     with torch.cuda.device(index):
         packed = w.new_empty(sh.lib().souffle_int8_packed_bytes(K, N))
-        sh.check(sh.lib().souffle_int8_pack_weight(w.data_ptr(), ld, packed.data_ptr(), K, N, sh.stream_of(index)))
+        sh.check(sh.lib().souffle_int8_pack_weight(w.data_ptr(), ld, packed.data_ptr(), K, N, _stream(index)))
     return Int8Weight(packed, scale.contiguous(), K, N)
 
 
@@ -122,7 +133,7 @@ def quantize_weight(weight):
         packed = w.new_empty(sh.lib().souffle_int8_packed_bytes(K, N), dtype=torch.int8)
         scale = w.new_empty(N, dtype=torch.float32)
         sh.check(sh.lib().souffle_int8_quantize_weight(w.data_ptr(), _DTYPES[w.dtype], ld, packed.data_ptr(), scale.data_ptr(), K, N,
-                                                       sh.stream_of(index)))
+                                                       _stream(index)))
     return Int8Weight(packed, scale, K, N)
 
 
@@ -132,7 +143,7 @@ def quantize_rows(x):
     index = _check_cuda("x", x)
     if x.dtype not in _DTYPES:
         raise TypeError("x must be float16, bfloat16 or float32")
-    if not sh.is_current(index):
+    if index != _device():
         with torch.cuda.device(index):
             return quantize_rows(x)
     x, ld = _rows("x", x)
@@ -140,7 +151,7 @@ def quantize_rows(x):
     ldq = -(-K // 64) * 64
     q = x.new_empty((M, ldq), dtype=torch.int8)
     scale = x.new_empty(M, dtype=torch.float32)
-    sh.check(sh.lib().souffle_quantize_rows(x.data_ptr(), _DTYPES[x.dtype], ld, q.data_ptr(), ldq, scale.data_ptr(), M, K, sh.stream_of(index)))
+    sh.check(sh.lib().souffle_quantize_rows(x.data_ptr(), _DTYPES[x.dtype], ld, q.data_ptr(), ldq, scale.data_ptr(), M, K, _stream(index)))
     return (q if K == ldq else q[:, :K]), scale
 
 
@@ -149,7 +160,7 @@ def gemm_int8(q, row_scale, weight, *, bias=None, act=None, dtype=torch.float16,
     multiples of 16 bytes and can be read up to K rounded up to 64 bytes (as quantize_rows and gated_norm_int8 make
     them; what lies behind K does not matter).  bias is of `dtype`; out: a [rows, N] tensor to write to."""
     index = _check_cuda("q", q)
-    if not sh.is_current(index):
+    if index != _device():
         with torch.cuda.device(index):
             return gemm_int8(q, row_scale, weight, bias=bias, act=act, dtype=dtype, out=out)
     _check_cuda("row_scale", row_scale, index)
@@ -170,7 +181,7 @@ def gemm_int8(q, row_scale, weight, *, bias=None, act=None, dtype=torch.float16,
     b, a = _epilogue(bias, act, N, dtype, index)
     out, ldy = _output(out, q, M, N, dtype, index)
     sh.check(sh.lib().souffle_gemm_int8(q.data_ptr(), ldq, row_scale.data_ptr(), packed, scale, b, a, out.data_ptr(), _DTYPES[dtype], ldy, M, N, K,
-                                        sh.stream_of(index)))
+                                        _stream(index)))
     return out
 
 
@@ -178,7 +189,7 @@ def linear_int8(x, weight, *, bias=None, act=None, out=None):
     """act(x . W + bias) with the rows of x [..., K] in 8 bits: quantize_rows and gemm_int8 in one call, bit for bit.
     Returns [rows, N] of x's type; bias is of that type too.  out must not overlap x."""
     index = _check_cuda("x", x)
-    if not sh.is_current(index):
+    if index != _device():
         with torch.cuda.device(index):
             return linear_int8(x, weight, bias=bias, act=act, out=out)
     if x.dtype not in _DTYPES:
@@ -193,9 +204,8 @@ def linear_int8(x, weight, *, bias=None, act=None, out=None):
     out, ldy = _output(out, x, M, N, x.dtype, index)
     if given:
         _check_apart(x, ld, out, ldy)
-    lib = sh.lib()
-    nbytes = lib.souffle_linear_int8_workspace_bytes(M, N, K)
+    nbytes = _workspace_bytes(M, N, K)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    sh.check(lib.souffle_linear_int8(x.data_ptr(), ld, packed, scale, b, a, out.data_ptr(), _DTYPES[x.dtype], ldy, M, N, K, sh.ptr(ws), nbytes,
-                                     sh.stream_of(index)))
+    sh.check(sh.lib().souffle_linear_int8(x.data_ptr(), ld, packed, scale, b, a, out.data_ptr(), _DTYPES[x.dtype], ldy, M, N, K, sh.ptr(ws), nbytes,
+                                          _stream(index)))
     return out

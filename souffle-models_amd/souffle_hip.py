@@ -210,17 +210,6 @@ def current_stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-def stream_of(index):
-    """hipStream_t of torch's current stream on device `index` (current_stream() builds a Stream object for it)."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-def is_current(index):
-    import torch
-    return torch._C._cuda_getDevice() == index
-
-
 class Workspace:
     """A zero-initialised device workspace, cached by the binding modules."""
 
