@@ -245,11 +245,14 @@ struct BwdArgs {
   int chunks_per_gate;              // > 0: that many chunks per gate row; 0: chunks hold whole gate rows
   int vectors, wanted;              // wanted: bit v set = the gradient of vector v goes to `partial`
   int wanted_gate;                  // the gate's gradient goes there or to dgate
+  int row_gates;                    // chunks hold whole gate rows of few rows each
   float a, post_eps, pre_eps;
 };
 
 // Several rows at a time (one per slot of TPR threads), slots in step, so that a barrier of the workgroup serves them all.
-template <class T, int TPR, int NV, int WG, RowForm FORM, bool KEEP>
+// Rows that share a gate row are taken in one go by all slots, or, where there are few of them (ROW_GATES), by one
+// slot each, which loads the gate with its row and writes the gate's gradient itself.
+template <class T, int TPR, int NV, int WG, RowForm FORM, bool KEEP, bool ROW_GATES>
 __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   typedef typename Vec8<T>::type V;
   constexpr int kSlots = WG / TPR;
@@ -305,18 +308,18 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   }
   // rows first .. end in runs that share a gate row
   for (int run = first; run < end;) {
-    const int gr = run / a.rows_per_gate, run_end = min((gr + 1) * a.rows_per_gate, end);
+    const int gr = run / a.rows_per_gate, run_end = ROW_GATES ? end : min((gr + 1) * a.rows_per_gate, end);
     V gt[NV], pg[NV], pb[NV], ng[NV];
     const void *gate = a.gate ? static_cast<const T *>(a.gate) + (long long)gr * n : nullptr;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = c0 + i * TPR * 8;
-      gt[i] = param_load<FORM, T>(gate, a.x, c, n);
+      if constexpr (!ROW_GATES) gt[i] = param_load<FORM, T>(gate, a.x, c, n);
       pg[i] = param_load<FORM, T>(a.post_gamma, a.x, c, n);
       pb[i] = param_load<FORM, T>(a.post_beta, a.x, c, n);
       ng[i] = param_load<FORM, T>(a.pre_gamma, a.x, c, n);
     }
-    V xv[NV], fv[NV], yv[NV], hv[NV];
+    V xv[NV], fv[NV], yv[NV], hv[NV], gv[NV];
     auto fetch = [&](int row) {      // (a slot without a row takes the run's first one, with gradients of zero)
       const bool valid = row < run_end;
       const long long r = valid ? row : run;
@@ -327,36 +330,43 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
         fv[i] = load_row<FORM>(static_cast<const T *>(a.f) + r * a.ldf, c, n);
         yv[i] = load_row<FORM>(dy + r * ld_dy, c, n);
         hv[i] = load_row<FORM>(dh + r * ld_dh, c, n);
+        if constexpr (ROW_GATES) gv[i] = load_row<FORM>(static_cast<const T *>(a.gate) + r / a.rows_per_gate * n, c, n);
       }
     };
-    if constexpr (KEEP) fetch(run + slot);
+    const int few = a.rows_per_gate, turns = ROW_GATES ? ((run_end - run) / few + kSlots - 1) / kSlots * few : (run_end - run + kSlots - 1) / kSlots;
+    auto row_of = [&](int turn) { return run + (ROW_GATES ? (turn / few * kSlots + slot) * few + turn % few : turn * kSlots + slot); };
+    if constexpr (KEEP) fetch(row_of(0));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = c0 + i * TPR * 8;
-      gt[i] = param_settle<FORM, T>(gt[i], gate, c, n, 1.f);
+      if constexpr (!ROW_GATES) gt[i] = param_settle<FORM, T>(gt[i], gate, c, n, 1.f);
       pg[i] = param_settle<FORM, T>(pg[i], a.post_gamma, c, n, 1.f);
       pb[i] = param_settle<FORM, T>(pb[i], a.post_beta, c, n, 0.f);
       ng[i] = param_settle<FORM, T>(ng[i], a.pre_gamma, c, n, 1.f);
     }
-    for (int base = run; base < run_end; base += kSlots) {
-      const int row = base + slot;
+    for (int turn = 0; turn < turns; ++turn) {
+      const int row = row_of(turn);
       const bool valid = row < run_end;
       float y[NV][8], fh[NV][8], d[NV][8], h[NV][8];
       if constexpr (!KEEP) {
         fetch(row);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) pg[i] = opaque(pg[i]), pb[i] = opaque(pb[i]), gt[i] = opaque(gt[i]);
+        for (int i = 0; i < NV; ++i) {
+          pg[i] = opaque(pg[i]), pb[i] = opaque(pb[i]);
+          if constexpr (!ROW_GATES) gt[i] = opaque(gt[i]);
+        }
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = c0 + i * TPR * 8;
+        if constexpr (ROW_GATES) gt[i] = settle_row<FORM, T>(gv[i], c, n);
         to_f32(y[i], settle_row<FORM, T>(xv[i], c, n));
         to_f32(fh[i], settle_row<FORM, T>(fv[i], c, n));
         to_f32(d[i], settle_row<FORM, T>(yv[i], valid && a.dy ? c : n, n));
         to_f32(h[i], settle_row<FORM, T>(hv[i], valid && a.dh ? c : n, n));
       }
       if constexpr (KEEP)
-        if (base + kSlots < run_end) fetch(row + kSlots);
+        if (turn + 1 < turns) fetch(row_of(turn + 1));
       float fr = 1.f;
       if (a.post != SOUFFLE_NORM_NONE) fr = normalize<FORM, TPR, NV>(fh, a.post, a.post_eps, n, c0, red);
 #pragma unroll
@@ -432,8 +442,18 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) store_row<FORM>(static_cast<T *>(a.df) + row * a.ld_df, c0 + i * TPR * 8, a.df && valid ? n : 0, from_f32<T>(d[i]));
+      if constexpr (ROW_GATES)
+        if (a.dgate && turn % few == few - 1) {      // the slot's rows of this gate row are done
+          T *dg = static_cast<T *>(a.dgate) + (long long)(row / few) * n;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            store_row<FORM>(dg, c0 + i * TPR * 8, valid ? n : 0, from_f32<T>(sums[kGate][i]));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sums[kGate][i][e] = 0.f;
+          }
+        }
     }
-    if (a.dgate && a.chunks_per_gate == 0) {      // the gate row's rows were all this workgroup's
+    if (!ROW_GATES && a.dgate && a.chunks_per_gate == 0) {      // the gate row's rows were all this workgroup's
       T *dg = static_cast<T *>(a.dgate) + (long long)gr * n;
       collect(1 << kGate, [&](int, int c, const float (&s)[8]) { store_row<FORM>(dg, c, n, from_f32<T>(s)); }, [&](int, int c, float s) { dg[c] = (T)s; });
 #pragma unroll
@@ -451,45 +471,50 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
 struct FinishArgs {
   const float *partial;
   void *out[kVectors];
-  int cols, vectors, wanted, chunks, chunks_per_gate;
+  int cols, vectors, wanted, chunks;
+  int chunks_per_gate;              // of each of the gate's rows
+  int others;                       // vectors except the gate
+  int vector_blocks;                // their workgroups
+  int gate_width;                   // columns of a workgroup of the gate's rows: 32, 128 or 1024
 };
-// Column sums over the chunks: 32 columns x 32 slices of the chunks per workgroup, slices added in order.  With 256 chunks a thread has
-// eight loads, all under way at once.
-template <class T>
-__global__ void __launch_bounds__(1024) k_gated_norm_grad_finish(const FinishArgs a) {
-  __shared__ float lds[32][33];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  int v = 0, seen = 0, first = 0, count = a.chunks;
-  long long row = 0;
-  // blockIdx.y: the wanted vectors in order, then the gate's further rows
-  int y = blockIdx.y;
-  if (y >= a.vectors) {
-    row = y - a.vectors + 1;
-    y = __popc(a.wanted & ((1 << kGate) - 1));
-  }
-  for (v = 0; v < kVectors; ++v)
-    if (a.wanted >> v & 1) {
-      if (seen == y) break;
-      ++seen;
-    }
-  if (v == kGate && a.chunks_per_gate > 0) {
-    first = (int)row * a.chunks_per_gate;
-    count = a.chunks_per_gate;
-  }
+// Column sums over the chunks, W columns x 1024 / W slices of the chunks per workgroup, slices added in order.  W is about the
+// largest that leaves a thread up to eight loads, all under way at once: 32 for the vectors' 256 chunks, more for a row of the
+// gate, which may have two chunks only (a workgroup per 32 columns of 128 gate rows x 4096 takes 27 us longer).
+template <class T, int W>
+__device__ __forceinline__ void finish_columns(const FinishArgs &a, float *lds, int v, int first, int count, int c0, long long row) {
+  constexpr int kSlices = 1024 / W;
+  const int lane = threadIdx.x % W, slice = threadIdx.x / W, c = c0 + lane;
   float s = 0.f;
   if (c < a.cols) {
-    const float *p = a.partial + ((long long)first * a.vectors + y) * a.cols + c;
+    const float *p = a.partial + ((long long)first * a.vectors + __popc(a.wanted & ((1 << v) - 1))) * a.cols + c;
 #pragma unroll 8
-    for (int k = slice; k < count; k += 32) s += p[(long long)k * a.vectors * a.cols];
+    for (int k = slice; k < count; k += kSlices) s += p[(long long)k * a.vectors * a.cols];
   }
-  lds[slice][lane] = s;
-  __syncthreads();
-  if (slice == 0 && c < a.cols) {
+  if constexpr (kSlices > 1) {
+    lds[slice * (W + 1) + lane] = s;
+    __syncthreads();
     s = 0.f;
+    if (slice == 0)
 #pragma unroll
-    for (int k = 0; k < 32; ++k) s += lds[k][lane];
-    static_cast<T *>(a.out[v])[row * a.cols + c] = (T)s;
+      for (int k = 0; k < kSlices; ++k) s += lds[k * (W + 1) + lane];
   }
+  if (slice == 0 && c < a.cols) static_cast<T *>(a.out[v])[row * a.cols + c] = (T)s;
+}
+template <class T>
+__global__ void __launch_bounds__(1024) k_gated_norm_grad_finish(const FinishArgs a) {
+  __shared__ float lds[1024 + 32];
+  int b = blockIdx.x;
+  if (b < a.vector_blocks) {      // the vectors take turns
+    int left = a.wanted & ~(1 << kGate);
+    for (int i = b % a.others; i > 0; --i) left &= left - 1;
+    finish_columns<T, 32>(a, lds, __ffs(left) - 1, 0, a.chunks, b / a.others * 32, 0);
+    return;
+  }
+  b -= a.vector_blocks;
+  const int blocks = (a.cols + a.gate_width - 1) / a.gate_width, row = b / blocks, c0 = b % blocks * a.gate_width, first = row * a.chunks_per_gate;
+  if (a.gate_width == 32) finish_columns<T, 32>(a, lds, kGate, first, a.chunks_per_gate, c0, row);
+  else if (a.gate_width == 128) finish_columns<T, 128>(a, lds, kGate, first, a.chunks_per_gate, c0, row);
+  else finish_columns<T, 1024>(a, lds, kGate, first, a.chunks_per_gate, c0, row);
 }
 
 // ------------------------------------------------------------------------------------------ host side ----
@@ -587,6 +612,9 @@ static Chunks plan_chunks(int rows, int rows_per_gate, int gate_grad, int want) 
   return c;
 }
 constexpr int kChunks = 256;      // one per CU
+// Gate rows of fewer rows than this are taken by one slot each.  Measured, us for 1 | 2 | 4 rows a gate row: 4096 x 512 fp16 15.9 | 14.9 | 18.2, by
+// all slots 53.2 | 30.7 | 20.1 (14.1 with 16 rows); 8192 x 4096 bf16 124 | 115 | 113 and 163 | 136 | 121 (105).
+constexpr int kFewRows = 8;
 
 static int wanted_vectors(const souffle_gated_norm_grad *g) {
   return (g->pre_gamma ? 1 << kPreGamma : 0) | (g->pre_beta ? 1 << kPreBeta : 0) | (g->gate ? 1 << kGate : 0) |
@@ -595,7 +623,8 @@ static int wanted_vectors(const souffle_gated_norm_grad *g) {
 
 template <RowForm FORM, class T, int TPR, int NV, int WG, bool KEEP = true>
 static int launch_bwd(const BwdArgs &a, int chunks, hipStream_t st) {
-  hipLaunchKernelGGL((k_gated_norm_grad<T, TPR, NV, WG, FORM, KEEP>), dim3(chunks), dim3(WG), 0, st, a);
+  if (a.row_gates) hipLaunchKernelGGL((k_gated_norm_grad<T, TPR, NV, WG, FORM, KEEP, true>), dim3(chunks), dim3(WG), 0, st, a);
+  else hipLaunchKernelGGL((k_gated_norm_grad<T, TPR, NV, WG, FORM, KEEP, false>), dim3(chunks), dim3(WG), 0, st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
@@ -613,8 +642,9 @@ static int backward(const BwdArgs &a, const FinishArgs &f, int gate_rows, hipStr
   const int rc = a.cols < 8 ? launch_bwd<kShort, T, 64, 1, 512>(a, f.chunks, st)
                             : a.cols % 8 ? rows_backward<kRagged, T>(a, f.chunks, st) : rows_backward<kWhole, T>(a, f.chunks, st);
   if (rc || f.vectors == 0) return rc;
-  const int more = (f.wanted >> kGate & 1) ? gate_rows - 1 : 0;
-  hipLaunchKernelGGL(k_gated_norm_grad_finish<T>, dim3((a.cols + 31) / 32, f.vectors + more), dim3(1024), 0, st, f);
+  const bool gate = f.wanted >> kGate & 1;
+  const int gate_blocks = gate ? gate_rows * ((f.cols + f.gate_width - 1) / f.gate_width) : 0;
+  hipLaunchKernelGGL(k_gated_norm_grad_finish<T>, dim3(f.vector_blocks + gate_blocks), dim3(1024), 0, st, f);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
@@ -698,7 +728,9 @@ extern "C" int souffle_gated_norm_backward(const souffle_gated_norm_cfg *c, cons
   }
   DeviceFacts df;
   if (int rc = device_facts(&df)) return rc;
-  const Chunks ch = plan_chunks(c->rows, rpg, g->gate != nullptr, kChunks);
+  // (whole gate rows to a chunk also where their gradient is not wanted, if a gate row's rows are few)
+  const bool few = w->gate && rpg < kFewRows;
+  const Chunks ch = plan_chunks(c->rows, rpg, g->gate || few, kChunks);
   const bool gate_direct = g->gate && ch.per_gate == 0;
   BwdArgs a = {};
   a.x = x; a.f = f; a.dy = dy; a.dh = dh;
@@ -711,8 +743,12 @@ extern "C" int souffle_gated_norm_backward(const souffle_gated_norm_cfg *c, cons
   a.wanted = gate_direct ? wanted & ~(1 << kGate) : wanted;
   a.vectors = __builtin_popcount(a.wanted);
   a.wanted_gate = g->gate != nullptr;
+  a.row_gates = few && ch.per_gate == 0;
   a.a = c->residual_scale; a.post_eps = c->post_eps; a.pre_eps = c->pre_eps;
-  FinishArgs fin = {static_cast<const float *>(ws), {g->pre_gamma, g->pre_beta, g->gate, g->post_gamma, g->post_beta}, c->cols, a.vectors, a.wanted, ch.count, ch.per_gate};
+  FinishArgs fin = {static_cast<const float *>(ws), {g->pre_gamma, g->pre_beta, g->gate, g->post_gamma, g->post_beta}, c->cols, a.vectors, a.wanted, ch.count, ch.per_gate, 0, 0, 0};
+  fin.others = __builtin_popcount(a.wanted & ~(1 << kGate));
+  fin.vector_blocks = fin.others * ((c->cols + 31) / 32);
+  fin.gate_width = ch.per_gate > 32 ? 32 : ch.per_gate > 8 ? 128 : 1024;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int gate_rows = c->rows / rpg;
   if (c->dtype == SOUFFLE_F16) return backward<half_t>(a, fin, gate_rows, st);

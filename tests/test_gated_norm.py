@@ -185,6 +185,42 @@ def test_many_rows(rows, cols, gate):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cols", [5, 40, 203, 1000, 1033, 2056, 4100, 8200])
+@pytest.mark.parametrize("gates,per_gate", [(300, 1), (261, 3), (256, 7), (257, 8), (90, 2)])
+def test_gradient_with_few_rows_per_gate(gates, per_gate, cols, dtype):
+    """Gate rows of one row and of several, more and fewer than there are chunks, the last chunk not full."""
+    announce("gated norm gradient %s %d gate rows of %d rows, %d columns" % (dtype, gates, per_gate, cols))
+    rows = gates * per_gate if cols < 4000 else min(gates, 258) * min(per_gate, 2)
+    gates = rows // (per_gate if cols < 4000 else min(per_gate, 2))
+    x, f, dy, dh = (values(20 + i, rows, cols, dtype=TYPES[dtype]) for i in range(4))
+    run_backward(dy, dh, x, f, params(25, rows, cols, TYPES[dtype], "layer", "rms", gates))
+
+
+@gpu
+@pytest.mark.parametrize("gates,rows,cols", [(128, 512, 1033), (2, 600, 40), (60, 600, 2100), (300, 600, 72)])
+def test_gate_rows_with_several_chunks_and_gradients_not_wanted(gates, rows, cols):
+    """Gate rows made of few and of many chunks; and the other gradients keep their bits where the gate's is not wanted
+    (its sums are then of other chunks: those of the vectors may differ, dx and df may not)."""
+    import gated_norm_binding as gn
+    announce("gated norm gradient %d gate rows of %d rows, %d columns" % (gates, rows, cols))
+    x, f, dy, dh = (values(40 + i, rows, cols) for i in range(4))
+    p = params(45, rows, cols, torch.float32, "rms", "layer", gates)
+    got = run_backward(dy, dh, x, f, p)
+    grads, bounds = ref.backward(dy, dh, x, f, p)
+    x, f, dy, dh, p = x.cuda(), f.cuda(), dy.cuda(), dh.cuda(), cuda(p)
+    dx, df, gamma = torch.empty_like(x), torch.empty_like(x), torch.empty(cols, device="cuda")
+    cfg = gn._cfg(rows, cols, sh.F32, sh.NORM_RMS, sh.NORM_LAYER, rows // gates, 0.75, 1e-5, 1e-6, cols, cols, cols, cols)
+    w = sh.GatedNormW(*[p[k].data_ptr() for k in ("post_gamma", "post_beta", "gate", "pre_gamma", "pre_beta")])
+    grad = sh.GatedNormGrad(dx.data_ptr(), df.data_ptr(), gamma.data_ptr(), None, None, None, None, cols, cols, cols, cols)
+    ws = torch.empty(sh.lib().souffle_gated_norm_backward_workspace_bytes(cfg), dtype=torch.uint8, device="cuda")
+    sh.check(sh.lib().souffle_gated_norm_backward(cfg, w, dy.data_ptr(), dh.data_ptr(), x.data_ptr(), f.data_ptr(), grad, ws.data_ptr(), ws.numel(),
+                                                  torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(dx, got["x"]) and torch.equal(df, got["f"])
+    ref.check("gradient of pre_gamma alone", gamma, grads["pre_gamma"], bounds["pre_gamma"])
+
+
+@gpu
 def test_one_incoming_gradient():
     announce("gated norm gradient: dy or dh alone")
     x, f, d = (values(i, 20, 72) for i in range(3))
