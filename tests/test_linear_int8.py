@@ -218,6 +218,30 @@ def test_linear_many_rows(M, K, N):
 
 
 @gpu
+@pytest.mark.parametrize("M", [1, 40, 4096])
+def test_gelu_keeps_its_digits_in_the_tails(M):
+    """Rows of zeros, so that the activation's argument is the bias itself.  Up to |v| = 4 the error is relative to the
+    result: the exponent, at most 8 log2(e), is rounded twice (9.5e-7 in the power), nine steps of a polynomial, four
+    products and two functions of one unit each add 9 + 4 + 4 roundings of 2^-24 and the fit 1e-7: 2.1e-6."""
+    import linear_int8_binding as lb
+    announce("gelu of %d rows" % M)
+    v = torch.cat([torch.linspace(-4, 4, 3000), torch.linspace(-30, 30, 1000), torch.logspace(-30, 30, 400), -torch.logspace(-30, 30, 400),
+                   torch.tensor([0.0, float("inf"), float("nan")])])
+    w = lb.quantize_weight(torch.ones(64, v.numel(), device="cuda"))
+    y = lb.linear_int8(torch.zeros(M, 64, device="cuda"), w, bias=v.cuda(), act="gelu").double().cpu()
+    assert torch.equal(y[:, :-1], y[:1, :-1].expand(M, -1))      # (without the NaN)
+    y, v = y[0], v.double()
+    assert y[-2] == float("inf") and torch.isnan(y[-1]) and y[-3] == 0
+    y, v = y[:-3], v[:-3]
+    exact = v.clamp_min(0) - 0.5 * v.abs() * torch.special.erfc(v.abs() / 2 ** 0.5)
+    error = (y - exact).abs()
+    near = v.abs() <= 4
+    # (v - w near 0 for positive v: the difference of the two is rounded, half a step of v)
+    assert (error[near] <= 2.1e-6 * exact[near].abs() + ref.EPS32 * v[near].clamp_min(0)).all()
+    assert (error <= 16 * ref.EPS32 * v.abs()).all()
+
+
+@gpu
 def test_longest_sums_stay_exact():
     """K = 131071 with every factor -128: the sum is 2147467264, 16384 short of what 32 bits hold."""
     announce("gemm_int8 K=131071")
