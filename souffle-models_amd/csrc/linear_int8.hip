@@ -237,25 +237,32 @@ __device__ __forceinline__ void finish4(const Args &a, int m, int n, i4 s, float
 // lines of the rows.  Bound by the arrival of the weights: 24 x 4096 -> 8192 takes 9.4 us, 34 MB at 3.6 TB/s (U = 2; with 3 or 4
 // steps asked for ahead 16 x 4096 -> 8192 takes 11.7 and 11.0 us instead of 10.3).
 //
-// ROWS: the rows come as activations, and every workgroup quantises all of them into LDS itself while its first weights
-// are under way: for a few rows that costs less than a launch of its own in front of this one.  (Not for the 32 rows of a wider
-// tile: 384 x 768 -> 768 takes 8.2 us that way and 6.6 in two launches; twelve workgroups repeat each row's work.)
+// ROWS: the rows come as activations, and every workgroup quantises its own into LDS itself while its first weights are under
+// way: that repeats the work for each tile of columns, but costs a call less than a launch of its own in front of this one.
+constexpr int kRowsK = 1024, kRowsPitch = kRowsK + 16;      // of tiles of 32 rows
+template <RowForm FORM>
+struct FormTag {
+  static constexpr RowForm value = FORM;
+};
 template <class T, int MF, int NF, int W, int U, bool ROWS>
 __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
   static_assert(4 % NF == 0, "operands of the four that 64 columns have");
-  static_assert(!ROWS || MF == 1, "rows of one operand");
   static_assert(MF * NF <= W, "four results per thread");
   constexpr int kParts = 4 / NF;
   __shared__ i4 lds[W][MF * NF][64];
-  __shared__ float lds_scale[16];
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds_rows[];      // ROWS: [M][64 kblocks + 16]
+  __shared__ float lds_scale[16 * MF];
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds_dynamic[];      // ROWS: [M][64 kblocks + 16]
+  __shared__ __attribute__((aligned(16))) unsigned char lds_static[ROWS && MF > 1 ? 16 * MF * kRowsPitch : 16];      // (more than 64 KB in all)
+  unsigned char *lds_rows = MF > 1 ? lds_static : lds_dynamic;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = blockIdx.x % a.col_tiles, group = col / kParts, t0 = col % kParts * NF, m0 = blockIdx.x / a.col_tiles * 16 * MF;
-  const int pitch = a.kblocks * 64 + 16;
+  const int pitch = a.kblocks * 64 + 16, rows_here = min(16 * MF, a.M - m0);
   i4 acc[MF][NF] = {};
   const int8_t *wp = a.packed + ((size_t)group * a.kblocks * 4 + t0) * 1024 + lane * 16;
   const int8_t *xp[MF];
-  const unsigned char *xrow = lds_rows + min(lane & 15, a.M - 1) * pitch + 16 * (lane >> 4);
+  const unsigned char *xrow[MF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i) xrow[i] = lds_rows + min(16 * i + (lane & 15), rows_here - 1) * pitch + 16 * (lane >> 4);
 #pragma unroll
   for (int i = 0; i < MF; ++i) xp[i] = a.q + min(m0 + 16 * i + (lane & 15), a.M - 1) * a.ldq + 16 * (lane >> 4);
   // U steps at a time, the next U loaded while the present ones are multiplied.  (A step behind the part's end reads its
@@ -283,7 +290,42 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
     columns.load(a, out_n);
     if constexpr (!ROWS) rs = a.row_scale[out_m];
   }
-  if constexpr (ROWS) {
+  if constexpr (ROWS && MF > 1) {
+    // every wave has its share of the rows (at most 1024 elements each), all asked for at once
+    constexpr int R = 16 * MF / W;
+    auto quantise = [&](auto form) {
+      constexpr RowForm FORM = decltype(form)::value;
+      typename Vec8<T>::type v[R][2];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          v[r][i] = load_row<FORM>(static_cast<const T *>(a.x) + (m0 + min(wave * R + r, rows_here - 1)) * a.ldx, (i * 64 + lane) * 8, a.K);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int row = wave * R + r;
+        float f[2][8];
+        unsigned m = 0u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          to_f32(f[i], settle_row<FORM, T>(v[r][i], (i * 64 + lane) * 8, a.K));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[i][e]));
+        }
+        const RowScale rs = row_scale(wave_umax_dpp(m));
+        if (row < rows_here) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if ((i * 64 + lane) * 8 < a.K) *reinterpret_cast<u2 *>(lds_rows + row * pitch + (i * 64 + lane) * 8) = quantize8(f[i], rs);
+          if (lane == 0) lds_scale[row] = rs.scale;
+        }
+      }
+    };
+    if (a.K % 8 == 0) quantise(FormTag<kWhole>());
+    else if (a.K > 8) quantise(FormTag<kRagged>());
+    else quantise(FormTag<kShort>());
+    __syncthreads();
+  } else if constexpr (ROWS) {
     // as many waves per row as there are for M rows at a time
     __shared__ unsigned lds_max[2][W];
     const int per_row = a.M == 1 ? W : a.M == 2 ? W / 2 : a.M <= 4 ? W / 4 : W / 8, slots = W / per_row;
@@ -332,7 +374,7 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
       for (int j = 0; j < NF; ++j) wn[u][j] = kb + u < k_end ? wv[u][j] : i4{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
-        if constexpr (ROWS) xn[u][i] = __builtin_bit_cast(i4, lds_load16(xrow + min(kb + u, k_end - 1) * 64));
+        if constexpr (ROWS) xn[u][i] = __builtin_bit_cast(i4, lds_load16(xrow[i] + min(kb + u, k_end - 1) * 64));
         else xn[u][i] = xv[u][i];
       }
     }
@@ -350,7 +392,7 @@ __global__ void __launch_bounds__(W * 64) k_gemm_split(const Args a) {
     for (int j = 0; j < NF; ++j) lds[wave][i * NF + j][lane] = acc[i][j];
   __syncthreads();
   if (!has_out) return;
-  if constexpr (ROWS) rs = lds_scale[out_m];
+  if constexpr (ROWS) rs = lds_scale[out_m - m0];
   i4 sum = lds[0][out_tile][lane];
 #pragma unroll
   for (int w = 1; w < W; ++w) sum += lds[w][out_tile][lane];
@@ -624,11 +666,11 @@ static int launch_split(Args a, hipStream_t st) {
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
-template <class T, int NF, int U>
+template <class T, int MF, int NF, int U>
 static int launch_rows(Args a, hipStream_t st) {
   unsigned grid;
-  if (int rc = grid_of(a, 16, 16 * NF, 512, &grid, &a.col_tiles)) return rc;
-  hipLaunchKernelGGL((k_gemm_split<T, 1, NF, 8, U, true>), dim3(grid), dim3(512), a.M * (a.kblocks * 64 + 16), st, a);
+  if (int rc = grid_of(a, 16 * MF, 16 * NF, 512, &grid, &a.col_tiles)) return rc;
+  hipLaunchKernelGGL((k_gemm_split<T, MF, NF, 8, U, true>), dim3(grid), dim3(512), MF > 1 ? 0 : a.M * (a.kblocks * 64 + 16), st, a);
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
@@ -668,15 +710,18 @@ static int gemm(const Args &a, int dtype, hipStream_t st) {
   if (dtype == SOUFFLE_BF16) return gemm<bf16_t>(a, st);
   return gemm<float>(a, st);
 }
-// Whether the product's workgroups quantise the rows themselves (one launch, no workspace): measured in one launch and in two, us,
-// 1 x 768 -> 2304 3.7 and 5.0, 2 x 4096 -> 8192 9.1 and 10.1, 4 x 4096 -> 4096 9.0 and 8.9, 8 x 4096 -> 4096 11.5 and 9.2, 16 x 1024 -> 4096
-// 6.0 and 6.0 (and some 4 us less on the host).
-static bool rows_in_kernel(int M, int K) {
-  return M <= 16 && (long long)M * K <= 16384;
+// Whether the product's workgroups quantise the rows themselves (one launch, no workspace).  Measured on the GPU in one launch and in
+// two, us: 1 x 768 -> 2304 3.7 and 5.0, 2 x 4096 -> 8192 9.1 and 10.1, 4 x 4096 -> 4096 9.0 and 8.9, 8 x 4096 -> 4096 11.5 and 9.2, 16 x 1024 ->
+// 4096 6.0 and 6.0; tiles of 32 rows: 32 x 512 -> 512 5.7 and 6.4, 384 x 768 -> 768 7.8 and 7.3, 128 x 1024 -> 4096 8.1 and 7.6, 333 x 1000 ->
+// 1111 fp32 8.4 and 7.7, 640 x 768 -> 768 7.7 and 7.7.  One call after another, which the host bounds, takes 8.8 and 12.9 in all of these.
+constexpr int kOneRound = 256;      // workgroups, one per CU: 98 KB of LDS each
+static bool rows_in_kernel(int M, int N, int K) {
+  return M <= 16 ? (long long)M * K <= 16384 : K <= kRowsK && tiles(M, 32, N, 64) <= kOneRound;
 }
 template <class T>
 static int linear_rows(const Args &a, hipStream_t st) {
-  return tiles(a.M, 16, a.N, 16) <= a.num_cus ? launch_rows<T, 1, 4>(a, st) : launch_rows<T, 4, 2>(a, st);
+  if (a.M > 16) return tiles(a.M, 32, a.N, 32) <= a.num_cus ? launch_rows<T, 2, 2, 2>(a, st) : launch_rows<T, 2, 4, 1>(a, st);
+  return tiles(a.M, 16, a.N, 16) <= a.num_cus ? launch_rows<T, 1, 1, 4>(a, st) : launch_rows<T, 1, 4, 2>(a, st);
 }
 
 static int check_product(const void *packed, const float *col_scale, const void *bias, int act, const void *y, int dtype, long long ldy, int M,
@@ -765,7 +810,7 @@ extern "C" int souffle_gemm_int8(const int8_t *q, long long ldq, const float *ro
 }
 
 extern "C" size_t souffle_linear_int8_workspace_bytes(int M, int N, int K) {
-  if (M < 0 || M > kMaxRows || check_kn(K, N) || rows_in_kernel(M, K)) return 0;
+  if (M < 0 || M > kMaxRows || check_kn(K, N) || rows_in_kernel(M, N, K)) return 0;
   return round_up((size_t)M * round_up(K, 64) + (size_t)M * 4, 256);
 }
 

@@ -218,6 +218,15 @@ def test_linear_many_rows(M, K, N):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(17, 3, 70), (31, 8, 64), (32, 9, 200), (33, 64, 33), (64, 511, 640), (100, 513, 1000), (250, 1000, 400), (384, 1023, 768),
+                                   (47, 1024, 4100), (300, 1025, 300), (640, 520, 832), (672, 520, 832)])
+def test_linear_rows_quantised_on_the_way(dtype, M, K, N):
+    """Tiles of 32 rows with their last rows missing, up to the longest row that is quantised there and one beyond."""
+    run_linear(dtype, M, K, N, "gelu", True, seed=M + K, ldx=K + 5)
+
+
+@gpu
 @pytest.mark.parametrize("M", [1, 40, 4096])
 def test_gelu_keeps_its_digits_in_the_tails(M):
     """Rows of zeros, so that the activation's argument is the bias itself.  Up to |v| = 4 the error is relative to the
