@@ -28,10 +28,11 @@ struct FwdArgs {
 // wave that writes half i again has passed the barrier of the sum in between, behind which nobody reads half i any more.
 template <int TPR>
 struct RowReduce {
-  static constexpr int kWaves = TPR / 64;
+  static constexpr int kWaves = TPR < 64 ? 1 : TPR / 64;
   unsigned *red;                    // [2][2 kWaves] of this row slot
   int turn;
   __device__ __forceinline__ float sum(float v) {
+    if constexpr (TPR == 16) return row16_sum_dpp(v);
     v = wave_sum_dpp(v);
     if constexpr (kWaves == 1) return v;
     float *r = reinterpret_cast<float *>(red) + turn * 2 * kWaves;
@@ -45,7 +46,8 @@ struct RowReduce {
   }
   // Two sums for one barrier.
   __device__ __forceinline__ void sum2(float &v0, float &v1) {
-    wave_sum2_dpp(v0, v1);
+    if constexpr (TPR == 16) v0 = row16_sum_dpp(v0), v1 = row16_sum_dpp(v1);
+    else wave_sum2_dpp(v0, v1);
     if constexpr (kWaves > 1) {
       float *r = reinterpret_cast<float *>(red) + turn * 2 * kWaves;
       turn ^= 1;
@@ -60,6 +62,7 @@ struct RowReduce {
     }
   }
   __device__ __forceinline__ unsigned umax(unsigned v) {
+    if constexpr (TPR == 16) return row16_umax_dpp(v);
     v = wave_umax_dpp(v);
     if constexpr (kWaves == 1) return v;
     unsigned *r = red + turn * 2 * kWaves;
@@ -135,11 +138,11 @@ __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
   typedef typename Vec8<T>::type V;
   constexpr int kSlots = WG / TPR;
   __shared__ __attribute__((aligned(16))) unsigned lds_red[WG / 64 * 4];
-  const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
-  RowReduce<TPR> red{lds_red + slot * 4 * RowReduce<TPR>::kWaves, 0};
+  const int slot = TPR < 64 ? threadIdx.x / TPR : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
+  RowReduce<TPR> red{lds_red + (TPR < 64 ? 0 : slot) * 4 * RowReduce<TPR>::kWaves, 0};
 
   const int first = (blockIdx.x * kSlots + slot) * a.rows_per_slot, end = min(first + a.rows_per_slot, a.rows);
-  if (TPR == 64 && first >= end) return;      // (rows of several waves: every workgroup has one)
+  if (TPR <= 64 && first >= end) return;      // (rows of several waves: every workgroup has one)
   V xv[NV], fv[NV];
   auto fetch = [&](int row) {
     const T *x = static_cast<const T *>(a.x) + row * a.ldx, *f = static_cast<const T *>(a.f) + row * a.ldf;
@@ -263,9 +266,9 @@ __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned lds_red[WG / 64 * 4];
   constexpr int kSlotCols = TPR * NV * 8;
   __shared__ __attribute__((aligned(16))) float lds_sum[kSlots > 1 ? kVectors * kSlots * kSlotCols : 1];
-  const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
+  const int slot = TPR < 64 ? threadIdx.x / TPR : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, c0 = t * 8, n = a.cols;
   const float inv_n = 1.0f / (float)n;
-  RowReduce<TPR> red{lds_red + slot * 4 * RowReduce<TPR>::kWaves, 0};
+  RowReduce<TPR> red{lds_red + (TPR < 64 ? 0 : slot) * 4 * RowReduce<TPR>::kWaves, 0};
 
   float sums[kVectors][NV][8] = {};
   // The sums of the vectors in `mask`, over the slots in their order: whole(v, c, eight of them) or one(v, c, sum).
@@ -565,8 +568,11 @@ static int launch_fwd(FwdArgs a, int num_cus, hipStream_t st) {
 template <RowForm FORM, class T>
 static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
   // One vector of 8 per thread in fp32, two in the 16-bit types from 513 elements on (measured: 4096 x 4096 fp32 48.6 us with one
-  // and 55.5 with two, which leave two waves per SIMD; 8192 x 4096 bf16 49.3 and 45.3, where two halve the waves of a sum).
+  // and 55.5 with two, which leave two waves per SIMD; 8192 x 4096 bf16 49.3 and 45.3, where two halve the waves of a sum).  Rows of up to
+  // 256 elements share a wave, 16 threads each: 262144 x 64 fp16 32 us (106 with 64 threads), 131072 x 256 fp16 45 (60), fp32 117 (114).
   if constexpr (sizeof(T) == 4) {
+    if (a.cols <= 128) return launch_fwd<FORM, T, 16, 1, 256>(a, num_cus, st);
+    if (a.cols <= 256) return launch_fwd<FORM, T, 16, 2, 256>(a, num_cus, st);
     if (a.cols <= 512) return launch_fwd<FORM, T, 64, 1, 256>(a, num_cus, st);
     if (a.cols <= 1024) return launch_fwd<FORM, T, 128, 1, 128>(a, num_cus, st);
     if (a.cols <= 2048) return launch_fwd<FORM, T, 256, 1, 256>(a, num_cus, st);
@@ -574,6 +580,8 @@ static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
     if (a.cols <= 8192) return launch_fwd<FORM, T, 1024, 1, 1024>(a, num_cus, st);
     return launch_fwd<FORM, T, 1024, 2, 1024>(a, num_cus, st);
   } else {
+    if (a.cols <= 128) return launch_fwd<FORM, T, 16, 1, 256>(a, num_cus, st);
+    if (a.cols <= 256) return launch_fwd<FORM, T, 16, 2, 256>(a, num_cus, st);
     if (a.cols <= 512) return launch_fwd<FORM, T, 64, 1, 256>(a, num_cus, st);
     if (a.cols <= 1024) return launch_fwd<FORM, T, 64, 2, 256>(a, num_cus, st);
     if (a.cols <= 2048) return launch_fwd<FORM, T, 256, 1, 256>(a, num_cus, st);
@@ -584,7 +592,7 @@ static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
 }
 template <class T>
 static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
-  if (a.cols < 8) return launch_fwd<kShort, T, 64, 1, 256>(a, num_cus, st);
+  if (a.cols < 8) return launch_fwd<kShort, T, 16, 1, 256>(a, num_cus, st);
   return a.cols % 8 ? forward<kRagged, T>(a, num_cus, st) : forward<kWhole, T>(a, num_cus, st);
 }
 
@@ -632,8 +640,11 @@ static int launch_bwd(const BwdArgs &a, int chunks, hipStream_t st) {
   SOUFFLE_HIP_TRY(hipGetLastError());
   return SOUFFLE_OK;
 }
+// (16 threads a row as in the forward pass: 262144 x 64 fp16 65 us, 235 with 64 threads; 131072 x 256 fp16 94 and 131, fp32 171 and 172)
 template <RowForm FORM, class T>
 static int rows_backward(const BwdArgs &a, int chunks, hipStream_t st) {
+  if (a.cols <= 128) return launch_bwd<FORM, T, 16, 1, 512>(a, chunks, st);
+  if (a.cols <= 256) return launch_bwd<FORM, T, 16, 2, 256>(a, chunks, st);
   if (a.cols <= 512) return launch_bwd<FORM, T, 64, 1, 512>(a, chunks, st);
   if (a.cols <= 1024) return launch_bwd<FORM, T, 128, 1, 512>(a, chunks, st);
   if (a.cols <= 2048) return launch_bwd<FORM, T, 256, 1, 512>(a, chunks, st);
@@ -643,7 +654,7 @@ static int rows_backward(const BwdArgs &a, int chunks, hipStream_t st) {
 }
 template <class T>
 static int backward(const BwdArgs &a, const FinishArgs &f, int gate_rows, hipStream_t st) {
-  const int rc = a.cols < 8 ? launch_bwd<kShort, T, 64, 1, 512>(a, f.chunks, st)
+  const int rc = a.cols < 8 ? launch_bwd<kShort, T, 16, 1, 512>(a, f.chunks, st)
                             : a.cols % 8 ? rows_backward<kRagged, T>(a, f.chunks, st) : rows_backward<kWhole, T>(a, f.chunks, st);
   if (rc || f.vectors == 0) return rc;
   const bool gate = f.wanted >> kGate & 1;

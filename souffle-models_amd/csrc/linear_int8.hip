@@ -38,7 +38,8 @@ __device__ __forceinline__ i4 ldg16(const int8_t *p) { return *(const __attribut
 // ---------------------------------------------------------------------------------------- quantisation ----
 // Rows: TPR threads per row, NV vectors of 8 per thread kept in registers between the largest value and the rounding
 // (NV = 0: any length, the row is read again for the rounding).  Bound by memory, 3 bytes per fp16 element: 8192 x 4096 bf16 takes 20 us,
-// 101 MB at 5.0 TB/s.  The thread count per row keeps one or two vectors a thread, so that small inputs spread over many waves.
+// 101 MB at 5.0 TB/s.  The thread count per row keeps one or two vectors a thread, so that small inputs spread over many waves, and
+// that rows of up to 128 elements share a wave (262144 x 64 fp16: 19 us with 16 threads a row, 58 with 64).
 template <class T, int TPR, int NV, RowForm FORM>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T *x, long long ldx, int8_t *q, long long ldq, float *scale, int rows, int cols) {
   constexpr int kSlots = 256 / TPR;
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T *x, long long ldx
         largest(f[0]);
       }
     }
-    m = wave_umax_dpp(m);
+    m = TPR == 16 ? row16_umax_dpp(m) : wave_umax_dpp(m);
     if constexpr (TPR > 64) {
       unsigned *r = lds_max[turn];
       if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = m;
@@ -628,7 +629,8 @@ constexpr int kMostRowGroups = 1 << 22;      // (a launch holds fewer than 2^32 
 template <RowForm FORM, class T>
 static void launch_quantize(const T *x, long long ldx, int8_t *q, long long ldq, float *scale, int M, int K, hipStream_t st) {
   const dim3 wide(std::min(M, kMostRowGroups)), narrow(std::min((M + 3) / 4, kMostRowGroups)), block(256);
-  if (K <= 512) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1, FORM>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
+  if (K <= 128) hipLaunchKernelGGL((k_quantize_rows<T, 16, 1, FORM>), dim3(std::min((M + 15) / 16, kMostRowGroups)), block, 0, st, x, ldx, q, ldq, scale, M, K);
+  else if (K <= 512) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1, FORM>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
   else if (K <= 1024) hipLaunchKernelGGL((k_quantize_rows<T, 64, 2, FORM>), narrow, block, 0, st, x, ldx, q, ldq, scale, M, K);
   else if (K <= 2048) hipLaunchKernelGGL((k_quantize_rows<T, 256, 1, FORM>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
   else if (K <= 4096) hipLaunchKernelGGL((k_quantize_rows<T, 256, 2, FORM>), wide, block, 0, st, x, ldx, q, ldq, scale, M, K);
@@ -638,7 +640,7 @@ static void launch_quantize(const T *x, long long ldx, int8_t *q, long long ldq,
 template <class T>
 static int quantize_rows(const void *xv, long long ldx, int8_t *q, long long ldq, float *scale, int M, int K, hipStream_t st) {
   const T *x = static_cast<const T *>(xv);
-  if (K < 8) hipLaunchKernelGGL((k_quantize_rows<T, 64, 1, kShort>), dim3(std::min((M + 3) / 4, kMostRowGroups)), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K);
+  if (K < 8) hipLaunchKernelGGL((k_quantize_rows<T, 16, 1, kShort>), dim3(std::min((M + 15) / 16, kMostRowGroups)), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K);
   else if (K % 8) launch_quantize<kRagged>(x, ldx, q, ldq, scale, M, K, st);
   else launch_quantize<kWhole>(x, ldx, q, ldq, scale, M, K, st);
   SOUFFLE_HIP_TRY(hipGetLastError());

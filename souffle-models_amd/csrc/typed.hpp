@@ -140,6 +140,22 @@ __device__ __forceinline__ void wave_sum2_dpp(float &v0, float &v1) {
   v0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 31));
   v1 = lane63(v);
 }
+// The same over each row of 16 lanes by rotations (every step adds two values that both lanes have, so all lanes get the same bits).
+__device__ __forceinline__ float row16_sum_dpp(float v) {
+  v += dpp<0x128, 15>(v, 0.f);      // row_ror:8
+  v += dpp<0x124, 15>(v, 0.f);
+  v += dpp<0x122, 15>(v, 0.f);
+  return v + dpp<0x121, 15>(v, 0.f);
+}
+__device__ __forceinline__ unsigned row16_umax_dpp(unsigned v) {
+#define SOUFFLE_STEP(CTRL) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 15, 15, false))
+  SOUFFLE_STEP(0x128);
+  SOUFFLE_STEP(0x124);
+  SOUFFLE_STEP(0x122);
+  SOUFFLE_STEP(0x121);
+#undef SOUFFLE_STEP
+  return v;
+}
 // Largest of non-negative floats or NaNs, as bit patterns: NaN > infinity > finite, so a NaN is never lost.
 __device__ __forceinline__ unsigned wave_umax_dpp(unsigned v) {
 #define SOUFFLE_STEP(CTRL, ROWS) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 15, false))

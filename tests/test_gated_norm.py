@@ -185,6 +185,29 @@ def test_many_rows(rows, cols, gate):
 
 
 @gpu
+@pytest.mark.parametrize("gate", [None, 7, "channel"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [1, 7, 16, 100, 128, 129, 200, 250, 256, 257])
+def test_rows_that_share_a_wave(cols, dtype, gate):
+    announce("gated norm %s of %d columns, gate=%s" % (dtype, cols, gate))
+    rows = 77 * 7
+    x, f, dy, dh = (values(60 + i, rows, cols, dtype=TYPES[dtype], mean=0.1) for i in range(4))
+    p = params(65, rows, cols, TYPES[dtype], "layer" if gate else "rms", "layer" if cols > 1 else "rms", gate)
+    x[5] = 0 if cols > 1 else x[5]
+    run_forward(x, f, p)
+    run_backward(dy, dh, x, f, p)
+    x[9] = float("nan")      # stays in its row
+    import gated_norm_binding as gn
+    y, h = gn.gated_norm(x.cuda(), f.cuda(), **cuda(p))
+    y8, q, s = gn.gated_norm_int8(x.cuda(), f.cuda(), **cuda(p))
+    g = gn.gated_norm_backward(dy.cuda(), dh.cuda(), x.cuda(), f.cuda(), **cuda(p))
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[9] = True
+    for v in (h.isnan().all(1), s.isnan(), g["x"].isnan().all(1)):
+        assert torch.equal(v, bad)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("cols", [5, 40, 203, 1000, 1033, 2056, 4100, 8200])
 @pytest.mark.parametrize("gates,per_gate", [(300, 1), (261, 3), (256, 7), (257, 8), (90, 2)])
