@@ -414,7 +414,8 @@ int souffle_quantize_rows(const void *x, int dtype, long long ldx, int8_t *q, lo
 int souffle_gemm_int8(const int8_t *q, long long ldq, const float *row_scale, const void *packed, const float *col_scale,
                       const void *bias, int act, void *y, int dtype, long long ldy, int M, int N, int K, souffle_stream_t stream);
 /* Both steps in one call, x [M][K] of `dtype`; same result, bit for bit.  The workspace holds the quantised rows during
- * the call and needs no initialisation; its size is 0 for a few rows, which the product's kernel quantises itself. */
+ * the call and needs no initialisation; its size is 0 where the product's kernel quantises the rows itself (few rows, or
+ * short ones that one round of workgroups holds). */
 size_t souffle_linear_int8_workspace_bytes(int M, int N, int K);
 int souffle_linear_int8(const void *x, long long ldx, const void *packed, const float *col_scale, const void *bias, int act, void *y,
                         int dtype, long long ldy, int M, int N, int K, void *workspace, size_t workspace_bytes, souffle_stream_t stream);

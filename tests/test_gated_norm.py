@@ -442,6 +442,68 @@ def test_block_and_gradient_in_a_graph_and_on_another_stream(rows):
 
 
 @gpu
+def test_calls_at_once_from_two_threads_and_two_graphs():
+    """Calls of different sizes on two streams at once, from two threads and as two captured graphs replayed side by side,
+    give what each gives alone."""
+    import threading
+
+    import gated_norm_binding as gn
+    import linear_int8_binding as lb
+    announce("two threads and two graphs at once")
+
+    def work(seed, rows, d, n):
+        x, f, dy, dh = (values(seed + i, rows, d, dtype=torch.float16).cuda() for i in range(4))
+        p = cuda(params(seed + 4, rows, d, torch.float16, "layer", "rms", "channel"))
+        w, b = lb.quantize_weight(values(seed + 9, d, n).cuda()), values(seed + 10, n, dtype=torch.float16).cuda()
+
+        def step():
+            y, q, s = gn.gated_norm_int8(x, f, **p)
+            z = lb.gemm_int8(q, s, w, bias=b, act="gelu")
+            z2 = lb.linear_int8(y, w, bias=b, act="relu")
+            g = gn.gated_norm_backward(dy, dh, x, f, **p)
+            return [y, q.contiguous(), s, z, z2] + [v for v in g.values() if v is not None]
+        return step
+    steps = [work(1, 300, 520, 700), work(31, 2000, 1100, 300)]
+    alone = [s() for s in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    wrong = []
+
+    def many(k):
+        try:
+            with torch.cuda.stream(streams[k]):
+                for _ in range(20):
+                    got = steps[k]()
+                    if not all(torch.equal(a, b) for a, b in zip(got, alone[k])):
+                        wrong.append(k)
+        except Exception as e:      # (a thread's own errors do not reach the test)
+            wrong.append(e)
+    threads = [threading.Thread(target=many, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g, s in zip(graphs, steps):
+        with torch.cuda.graph(g):
+            outs.append(s())
+    for turn in range(4):
+        for out in outs:
+            for v in out:
+                v.zero_()
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        eager = steps[turn % 2]()      # and the same work beside them
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(outs[k], alone[k])), "graph %d, replay %d" % (k, turn)
+        assert all(torch.equal(a, b) for a, b in zip(eager, alone[turn % 2]))
+
+
+@gpu
 def test_post_norm_encoder_form():
     """LN(x + f) of a post-norm encoder: no norm behind the block, no gate, y not kept."""
     announce("gated norm as LN(x + f)")
