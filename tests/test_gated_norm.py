@@ -308,6 +308,80 @@ def test_rows_apart_in_place_and_what_lies_around():
                 assert torch.equal(now, old), "written outside the rows"
 
 
+# (type, rows, columns, gate rows): more rows than the forward launch has slots for, so that a slot walks over two or three of them, for every
+# count of threads per row; an odd number of rows per gate row, so that its border falls inside a slot's run.
+WALKS = [("f16", 33000, 7, 40), ("f32", 33000, 40, 40), ("bf16", 70000, 24, 16), ("f16", 33000, 250, 40), ("bf16", 9000, 300, 8), ("f16", 8200, 520, 8),
+         ("f32", 4100, 1001, 4), ("bf16", 2100, 1100, 4), ("f32", 2100, 1104, 4), ("f16", 2100, 2056, 4), ("f32", 1030, 2056, 2), ("bf16", 1030, 4104, 2),
+         ("f32", 1100, 4099, 4), ("f16", 520, 8200, 8), ("f32", 520, 8200, 8)]
+
+
+def threads_per_row(dtype, cols):
+    """Of the forward kernel."""
+    if dtype == "f32":
+        return next(t for t, most in ((16, 256), (64, 512), (128, 1024), (256, 2048), (512, 4096), (1024, 16384)) if cols <= most)
+    return next(t for t, most in ((16, 256), (64, 1024), (256, 4096), (512, 8192), (1024, 16384)) if cols <= most)
+
+
+def abi(x, p, gates):
+    """(cfg, vectors, (ld, dtype)) of the C calls on contiguous rows like x's with the keywords p."""
+    rows, cols = x.shape
+    kinds = {None: sh.NORM_NONE, "layer": sh.NORM_LAYER, "rms": sh.NORM_RMS}
+    c = sh.GatedNormCfg(rows, cols, {torch.float16: sh.F16, torch.bfloat16: sh.BF16, torch.float32: sh.F32}[x.dtype], kinds[p["post_norm"]], kinds[p["pre_norm"]],
+                        rows // gates if gates else 0, p["residual_scale"], p["post_eps"], p["pre_eps"], cols, cols, cols, cols)
+    return c, sh.GatedNormW(*(sh.ptr(p.get(n)) for n in ("post_gamma", "post_beta", "gate", "pre_gamma", "pre_beta")))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,rows,cols,gates", WALKS)
+def test_forward_walks_over_several_rows(dtype, rows, cols, gates):
+    """The next row asked for while the present one is reduced, the gate changed on the way: against 64 bits, and in place."""
+    import gated_norm_binding as gn
+    announce("gated norm %s %dx%d, %d gate rows: several rows a slot" % (dtype, rows, cols, gates))
+    slots = sh.device_info()["num_cus"] * 2048 // threads_per_row(dtype, cols)
+    per_slot = -(-rows // slots)
+    assert per_slot > 1 and rows // gates % per_slot, "this case does not test what it is for"
+    x, f = values(70, rows, cols, dtype=TYPES[dtype], std=2.0, mean=0.1), values(71, rows, cols, dtype=TYPES[dtype])
+    post, pre = [("layer", "rms"), ("rms", "layer"), (None, "layer"), ("layer", "layer")][cols % 4]
+    p = params(72, rows, cols, TYPES[dtype], post, pre, gates)
+    run_forward(x, f, p)
+    x, f, p = x.cuda(), f.cuda(), cuda(p)
+    y, h = gn.gated_norm(x, f, **p)
+    for over in ((0, 1), (1, 0)):      # y over x and h over f, and the other way round
+        a = [x.clone(), f.clone()]
+        c, w = abi(x, p, gates)
+        sh.check(sh.lib().souffle_gated_norm_forward(C.byref(c), C.byref(w), a[0].data_ptr(), a[1].data_ptr(), a[over[0]].data_ptr(), a[over[1]].data_ptr(),
+                                                     sh.current_stream()))
+        torch.cuda.synchronize()
+        assert torch.equal(a[over[0]], y) and torch.equal(a[over[1]], h)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,rows,cols,gates", [("f32", 3001, 200, None), ("bf16", 2100, 1001, None), ("f16", 6000, 64, 8), ("f16", 515, 300, 515), ("f32", 783, 520, 261),
+                                                   ("bf16", 90, 2100, 90), ("f16", 600, 4100, 4), ("f32", 520, 5000, None), ("f32", 300, 8200, 300), ("bf16", 270, 8200, 1)])
+def test_gradient_in_place(dtype, rows, cols, gates):
+    """dx over dy and df over dh gives the bits of outputs of their own: slots without a row, several turns, a gate row a token, wide rows."""
+    announce("gated norm gradient in place %s %dx%d, gate rows: %s" % (dtype, rows, cols, gates))
+    x, f, dy, dh = (values(80 + i, rows, cols, dtype=TYPES[dtype]).cuda() for i in range(4))
+    p = cuda(params(85, rows, cols, TYPES[dtype], "layer", "layer" if gates else "rms", gates or "channel"))
+    c, w = abi(x, p, gates)
+    names = ("pre_gamma", "pre_beta", "gate", "post_gamma", "post_beta")
+    ws = torch.empty(sh.lib().souffle_gated_norm_backward_workspace_bytes(C.byref(c)), dtype=torch.uint8, device="cuda")
+
+    def call(dx, df, dy, dh):
+        vectors = [torch.empty_like(p[n]) for n in names]
+        grad = sh.GatedNormGrad(dx.data_ptr(), df.data_ptr(), *(v.data_ptr() for v in vectors), cols, cols, cols, cols)
+        sh.check(sh.lib().souffle_gated_norm_backward(C.byref(c), C.byref(w), sh.ptr(dy), sh.ptr(dh), x.data_ptr(), f.data_ptr(), C.byref(grad), ws.data_ptr(),
+                                                      ws.numel(), sh.current_stream()))
+        return [dx, df] + vectors
+    for given in ((dy, dh), (dy, None), (None, dh)):
+        apart = call(torch.empty_like(x), torch.empty_like(x), *given)
+        mine = [None if d is None else d.clone() for d in given]
+        over = call(*(torch.empty_like(x) if d is None else d for d in mine), *mine)
+        torch.cuda.synchronize()
+        for name, a, b in zip(("x", "f") + names, apart, over):
+            assert torch.isfinite(a).all() and torch.equal(a, b), name
+
+
 @gpu
 def test_hard_rows():
     """Constant rows, zero rows, a mean a thousand times the deviation; NaN and infinity stay in their rows."""
