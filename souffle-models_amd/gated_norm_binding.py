@@ -12,8 +12,9 @@ of all three:
     gate                    [D], or [G, D]: one row for each of G equal runs of rows (a sequence), or None
     residual_scale, post_eps, pre_eps               numbers
 Statistics and sums are in fp32, h comes from y before y is rounded, and two calls give the same bits.  Work is queued on
-the current stream of the tensors' device and nothing is kept between calls.  Autograd does not record these calls:
-a training step calls gated_norm_backward (or an autograd function around the two does).
+the current stream of the tensors' device and nothing is kept between calls.  Where gradients are on and an input
+requires one, autograd records gated_norm, and its backward pass is gated_norm_backward; that pass cannot be captured into a
+graph through autograd (gated_norm_backward itself can).  gated_norm_int8 is not recorded.
 """
 import ctypes as C
 import functools
@@ -102,15 +103,46 @@ def _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_ep
     return x, f, index, cfg, w
 
 
+class _Recorded(torch.autograd.Function):
+    """gated_norm for autograd: `call` makes (y, h), `numbers` are the keywords that are no tensors."""
+
+    @staticmethod
+    def forward(ctx, call, numbers, x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta):
+        ctx.numbers = numbers
+        ctx.set_materialize_grads(False)      # (None for an output that the loss does not use)
+        ctx.save_for_backward(x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta)
+        return call()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        # What autograd adds to a captured pass (the leaves' accumulation, on the streams of eager graphs that are still there) may end the process.
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("autograd's backward pass through gated_norm cannot be captured into a graph: capture gated_norm_backward")
+        x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta = ctx.saved_tensors
+        dy, dh = (None if d is None else d.contiguous() for d in (dy, dh))      # (a sum's gradient is one element, expanded)
+        g = gated_norm_backward(dy, dh, x, f, gate=gate, post_gamma=post_gamma, post_beta=post_beta, pre_gamma=pre_gamma, pre_beta=pre_beta, **ctx.numbers)
+        return (None, None) + tuple(g[name] for name in ("x", "f", "gate", "post_gamma", "post_beta", "pre_gamma", "pre_beta"))
+
+
 @_on_device(0)
 def gated_norm(x, f, *, gate=None, residual_scale=1.0, post_norm="layer", post_gamma=None, post_beta=None, post_eps=1e-5,
                pre_norm="layer", pre_gamma=None, pre_beta=None, pre_eps=1e-5, want_y=True):
-    """(y, h), of x's shape and type; y is None with want_y=False (a post-norm encoder only keeps h)."""
+    """(y, h), of x's shape and type; y is None with want_y=False (a post-norm encoder only keeps h).  Differentiable."""
     xr, fr, index, cfg, w = _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_eps, pre_norm, pre_gamma, pre_beta, pre_eps)
-    y = _like(x) if want_y else None
-    h = _like(x)
-    sh.check(sh.lib().souffle_gated_norm_forward(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), h.data_ptr(), _stream(index)))
-    return y, h
+
+    def call():
+        y = _like(x) if want_y else None
+        h = _like(x)
+        sh.check(sh.lib().souffle_gated_norm_forward(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), h.data_ptr(), _stream(index)))
+        return y, h
+    if torch.is_grad_enabled():
+        tensors = (x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta)
+        for v in tensors:
+            if v is not None and v.requires_grad:
+                numbers = dict(residual_scale=residual_scale, post_norm=post_norm, post_eps=post_eps, pre_norm=pre_norm, pre_eps=pre_eps)
+                return _Recorded.apply(call, numbers, *tensors)
+    return call()
 
 
 @_on_device(0)

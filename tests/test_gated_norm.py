@@ -278,6 +278,81 @@ def test_gradients_against_differences(post, pre, gate):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("post,pre,gate", [("layer", "layer", "channel"), ("rms", "rms", 3), (None, "layer", 6), ("layer", "rms", None)])
+def test_autograd_gives_the_gradient(dtype, post, pre, gate):
+    """loss.backward() through gated_norm is gated_norm_backward, bit for bit, with and without another path to the loss."""
+    import gated_norm_binding as gn
+    announce("gated norm by autograd: %s %s %s %s" % (dtype, post, pre, gate))
+    t = TYPES[dtype]
+    x, f, dy, dh = (values(90 + i, 2, 3, 72, dtype=t).cuda() for i in range(4))
+    p = cuda(params(95, 6, 72, t, post, pre, gate))
+    leaves = {"x": x, "f": f, **{k: v for k, v in p.items() if isinstance(v, torch.Tensor)}}
+    expect = gn.gated_norm_backward(dy, dh, x, f, **p)
+    plain = gn.gated_norm(x, f, **p)
+    assert not plain[0].requires_grad and not plain[1].requires_grad
+    for v in leaves.values():
+        v.requires_grad_(True)
+    with torch.no_grad():
+        assert not gn.gated_norm(x, f, **p)[1].requires_grad
+    y, h = gn.gated_norm(x, f, **p)
+    assert torch.equal(y, plain[0]) and torch.equal(h, plain[1]) and y.requires_grad and h.requires_grad
+    for name, got in zip(leaves, torch.autograd.grad([y, h], list(leaves.values()), [dy, dh], retain_graph=True)):
+        assert got.dtype == t and torch.equal(got, expect[name]), name
+    y.backward(dy, retain_graph=True)      # one output alone, accumulated into the leaves
+    alone = gn.gated_norm_backward(dy, None, x.detach(), f.detach(), **{k: v.detach() if isinstance(v, torch.Tensor) else v for k, v in p.items()})
+    for name, v in leaves.items():
+        assert torch.equal(v.grad, alone[name]), name
+        v.grad = None
+    (h * dh).sum().backward()
+    alone = gn.gated_norm_backward(None, dh, x.detach(), f.detach(), **{k: v.detach() if isinstance(v, torch.Tensor) else v for k, v in p.items()})
+    for name, v in leaves.items():
+        assert torch.equal(v.grad, alone[name]), name
+    # beside another path, the expanded gradient of a sum, y not wanted, and only some inputs that require a gradient
+    f, frozen = f.detach(), {k: v.detach() if isinstance(v, torch.Tensor) else v for k, v in p.items()}
+    x.grad = None
+    _, h = gn.gated_norm(x, f, **frozen, want_y=False)
+    assert _ is None
+    (h.sum() + x.sum()).backward()
+    one = torch.ones_like(x)
+    assert torch.equal(x.grad, one + gn.gated_norm_backward(None, one, x.detach(), f, **frozen)["x"])
+
+
+@gpu
+def test_autograd_refuses_what_it_cannot_do():
+    """A second derivative, inputs written over before the backward pass, and a captured backward pass; the leaves stay usable."""
+    import gated_norm_binding as gn
+    announce("gated norm by autograd: refusals")
+    x, f, d = (values(i, 6, 72).cuda() for i in range(3))
+    x.requires_grad_(True)
+    y, h = gn.gated_norm(x, f)
+    first, = torch.autograd.grad(h, x, d, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), x)
+    y, h = gn.gated_norm(x, f)
+    f.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.backward(d)
+    expect = gn.gated_norm(x.detach(), f)[1]
+    kept = gn.gated_norm(x, f)      # an eager graph of the same leaf stays alive
+    x.grad = None
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        _, held = gn.gated_norm(x, f)
+        with pytest.raises(RuntimeError, match="capture gated_norm_backward"):
+            held.backward(d)
+    assert x.grad is None
+    for _ in range(3):
+        held.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, expect)
+    kept[1].backward(d)
+    assert torch.equal(x.grad, gn.gated_norm_backward(None, d, x.detach(), f)["x"])
+
+
+@gpu
 def test_rows_apart_in_place_and_what_lies_around():
     """Slices of wider tensors that start anywhere as inputs; through the C ABI: y over x and h over f in place, outputs in
     rows apart, columns and rows around them left as they were."""
