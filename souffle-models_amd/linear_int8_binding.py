@@ -8,7 +8,7 @@
 A row x is held as q = round_half_even(x / s), s = max(max|x| / 127, 2^-100) in fp32, a weight column likewise; products
 sum in exact 32-bit integers.  A row with a NaN or an infinity gives a row of NaN.  Work is queued on the current
 stream of the tensors' device; nothing is kept between calls, so calls may overlap on several streams and be captured.
-Autograd does not record these calls.
+They are for inference: autograd does not record them, so their results require no gradient, whatever x requires.
 """
 import functools
 from typing import NamedTuple
@@ -98,14 +98,30 @@ def _output(out, like, rows, n, dtype, index):
     return _rows("out", out)
 
 
-def _check_apart(x, ldx, out, ldy):
-    """The rows of x and of out, both of one type, have no element in common (some are still read when others are written)."""
-    size, a, b = x.element_size(), x.data_ptr(), out.data_ptr()
-    if not x.numel() or a + ((x.shape[0] - 1) * ldx + x.shape[1]) * size <= b or b + ((out.shape[0] - 1) * ldy + out.shape[1]) * size <= a:
-        return
-    gap = (b - a) % (ldx * size)
-    if ldx != ldy or gap < x.shape[1] * size or gap + out.shape[1] * size > ldx * size:      # (else: columns side by side in one buffer)
-        raise ValueError("out must not overlap x")
+def _overlap(a, rows_a, width_a, pitch_a, b, rows_b, width_b, pitch_b):
+    """Whether two sets of rows have a byte in common (address, rows, bytes of a row, distance of the rows).  Sets that lie within
+    each other count as apart only where their rows do as columns side by side in one buffer."""
+    if not rows_a or not rows_b or a + (rows_a - 1) * pitch_a + width_a <= b or b + (rows_b - 1) * pitch_b + width_b <= a:
+        return False
+    if rows_a == 1:
+        pitch_a = pitch_b
+    if rows_b == 1:
+        pitch_b = pitch_a
+    gap = (b - a) % pitch_a
+    return pitch_a != pitch_b or gap < width_a or gap + width_b > pitch_a
+
+
+def _check_apart(name, rows, ld, out, ldy, weight, bias, row_scale=None):
+    """out has no byte in common with an input (some are still read when it is written): the rows named `name`, row_scale, bias, weights."""
+    size, (M, N) = out.element_size(), out.shape
+    wide = rows.element_size()
+    if _overlap(rows.data_ptr(), rows.shape[0], rows.shape[1] * wide, ld * wide, out.data_ptr(), M, N * size, ldy * size):
+        raise ValueError("out must not overlap " + name)
+    for name, t in (("row_scale", row_scale), ("bias", bias), ("weight.packed", weight.packed), ("weight.scale", weight.scale)):
+        if t is not None:
+            nbytes = t.numel() * t.element_size()
+            if _overlap(t.data_ptr(), 1, nbytes, nbytes, out.data_ptr(), M, N * size, ldy * size):
+                raise ValueError("out must not overlap " + name)
 
 
 def pack_weight(weight_q, scale):
@@ -158,7 +174,7 @@ def quantize_rows(x):
 def gemm_int8(q, row_scale, weight, *, bias=None, act=None, dtype=torch.float16, out=None):
     """act(row_scale * weight.scale * (q . W) + bias) as [rows, N] of `dtype`.  q [rows, K] int8: rows that start at
     multiples of 16 bytes and can be read up to K rounded up to 64 bytes (as quantize_rows and gated_norm_int8 make
-    them; what lies behind K does not matter).  bias is of `dtype`; out: a [rows, N] tensor to write to."""
+    them; what lies behind K does not matter).  bias is of `dtype`; out: a [rows, N] tensor to write to, apart from all inputs."""
     index = _check_cuda("q", q)
     if index != _device():
         with torch.cuda.device(index):
@@ -179,7 +195,10 @@ def gemm_int8(q, row_scale, weight, *, bias=None, act=None, dtype=torch.float16,
     if M > 0 and q.untyped_storage().nbytes() < q.storage_offset() + (M - 1) * ldq + need:
         raise ValueError("the rows of q must be readable up to %d bytes each (quantize_rows makes such rows)" % need)
     b, a = _epilogue(bias, act, N, dtype, index)
+    given = out is not None
     out, ldy = _output(out, q, M, N, dtype, index)
+    if given:
+        _check_apart("q", q, ldq, out, ldy, weight, bias, row_scale)
     sh.check(sh.lib().souffle_gemm_int8(q.data_ptr(), ldq, row_scale.data_ptr(), packed, scale, b, a, out.data_ptr(), _DTYPES[dtype], ldy, M, N, K,
                                         _stream(index)))
     return out
@@ -187,7 +206,7 @@ def gemm_int8(q, row_scale, weight, *, bias=None, act=None, dtype=torch.float16,
 
 def linear_int8(x, weight, *, bias=None, act=None, out=None):
     """act(x . W + bias) with the rows of x [..., K] in 8 bits: quantize_rows and gemm_int8 in one call, bit for bit.
-    Returns [rows, N] of x's type; bias is of that type too.  out must not overlap x."""
+    Returns [rows, N] of x's type; bias is of that type too.  out must not overlap an input."""
     index = _check_cuda("x", x)
     if index != _device():
         with torch.cuda.device(index):
@@ -203,7 +222,7 @@ def linear_int8(x, weight, *, bias=None, act=None, out=None):
     given = out is not None
     out, ldy = _output(out, x, M, N, x.dtype, index)
     if given:
-        _check_apart(x, ld, out, ldy)
+        _check_apart("x", x, ld, out, ldy, weight, bias)
     nbytes = _workspace_bytes(M, N, K)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     sh.check(sh.lib().souffle_linear_int8(x.data_ptr(), ld, packed, scale, b, a, out.data_ptr(), _DTYPES[x.dtype], ldy, M, N, K, sh.ptr(ws), nbytes,

@@ -76,6 +76,65 @@ def test_bindings_refuse_cpu_tensors():
             call()
 
 
+def test_overlap_of_rows():
+    """Against the sets of bytes themselves.  Rows at one distance whose columns meet count as overlapping wherever the spans do, which
+    is more than the bytes say only where one set begins behind the other's last row, or the distances differ."""
+    import linear_int8_binding as lb
+
+    def touched(a, rows, width, pitch):
+        return {a + r * pitch + c for r in range(rows) for c in range(width)}
+    for rows_a, width_a, pitch_a in ((0, 3, 8), (1, 5, 5), (3, 3, 8), (2, 8, 8)):
+        for rows_b, width_b, pitch_b in ((1, 2, 2), (1, 20, 20), (3, 4, 8), (3, 3, 8), (2, 3, 7)):
+            for b in range(60, 140):
+                both = touched(100, rows_a, width_a, pitch_a) & touched(b, rows_b, width_b, pitch_b)
+                got = lb._overlap(100, rows_a, width_a, pitch_a, b, rows_b, width_b, pitch_b)
+                assert got or not both, (rows_a, width_a, rows_b, width_b, b)
+                if got and not both:
+                    spans = rows_a and 100 < b + (rows_b - 1) * pitch_b + width_b and b < 100 + (rows_a - 1) * pitch_a + width_a
+                    assert spans and (pitch_a != pitch_b or rows_a != rows_b), (rows_a, width_a, rows_b, width_b, b)
+    # columns side by side, and one row in the gap between another's rows
+    assert not lb._overlap(100, 5, 16, 64, 116, 5, 48, 64) and not lb._overlap(116, 5, 48, 64, 100, 5, 16, 64) and lb._overlap(100, 5, 16, 64, 115, 5, 16, 64)
+    assert not lb._overlap(120, 1, 30, 30, 100, 5, 16, 64) and lb._overlap(120, 1, 50, 50, 100, 5, 16, 64)
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 3, 200])
+def test_out_over_an_input_is_refused(M):
+    """The product reads all of its inputs while it writes: out over the 8-bit rows, a scale, the bias or the weights."""
+    announce("8-bit product: out over an input, M=%d" % M)
+    import linear_int8_binding as lb
+    w = lb.quantize_weight(values(3, 64, 64).cuda())
+    x, b = values(4, M, 64).cuda(), values(5, 64).cuda()
+    room = torch.zeros(M * 320, dtype=torch.uint8, device="cuda")
+    q = room[:M * 64].view(torch.int8).view(M, 64)
+    q0, s = lb.quantize_rows(x)
+    q.copy_(q0)
+    y = lb.gemm_int8(q, s, w, bias=b, dtype=torch.float32)
+    over = lambda at: room[at:at + M * 256].view(torch.float32).view(M, 64)  # noqa: E731
+    with pytest.raises(ValueError, match="overlap q"):
+        lb.gemm_int8(q, s, w, bias=b, dtype=torch.float32, out=over(0))
+    with pytest.raises(ValueError, match="overlap q"):
+        lb.gemm_int8(q, s, w, bias=b, dtype=torch.float32, out=over(M * 64 - 4))
+    assert torch.equal(lb.gemm_int8(q, s, w, bias=b, dtype=torch.float32, out=over(M * 64)), y)
+    out = torch.empty(M, 64, device="cuda")
+    inside = out.view(-1)
+    packed = torch.empty(4096 + M * 256, dtype=torch.int8, device="cuda")
+    packed[:4096] = w.packed
+    bad = [("bias", w, inside[:64], out), ("weight.scale", w._replace(scale=inside[-64:]), b, out),
+           ("weight.packed", w._replace(packed=packed[:4096]), b, packed[4092:4092 + M * 256].view(torch.float32).view(M, 64))]
+    for name, weight, bias, o in bad:
+        with pytest.raises(ValueError, match="overlap " + name):
+            lb.gemm_int8(q, s, weight, bias=bias, dtype=torch.float32, out=o)
+        with pytest.raises(ValueError, match="overlap " + name):
+            lb.linear_int8(x, weight, bias=bias, out=o)
+    with pytest.raises(ValueError, match="overlap row_scale"):
+        lb.gemm_int8(q, inside[:M], w, bias=b, dtype=torch.float32, out=out)
+    # inputs between the rows of an output that lie apart are fine
+    wide = torch.zeros(M, 192, device="cuda")
+    wide[0, 64:128] = b
+    assert torch.equal(lb.linear_int8(x, w, bias=wide[0, 64:128], out=wide[:, 128:]), y) and torch.equal(wide[0, 64:128], b)
+
+
 @gpu
 def test_bindings_refuse_wrong_tensors():
     announce("8-bit linear layer: refusals of the bindings")
