@@ -104,14 +104,14 @@ def _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_ep
 
 
 class _Recorded(torch.autograd.Function):
-    """gated_norm for autograd: `call` makes (y, h), `numbers` are the keywords that are no tensors."""
+    """gated_norm for autograd; `numbers` are the keywords that are no tensors."""
 
     @staticmethod
-    def forward(ctx, call, numbers, x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta):
+    def forward(ctx, want_y, numbers, x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta):
         ctx.numbers = numbers
         ctx.set_materialize_grads(False)      # (None for an output that the loss does not use)
         ctx.save_for_backward(x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta)
-        return call()
+        return gated_norm(x, f, gate=gate, post_gamma=post_gamma, post_beta=post_beta, pre_gamma=pre_gamma, pre_beta=pre_beta, want_y=want_y, **numbers)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -130,19 +130,15 @@ def gated_norm(x, f, *, gate=None, residual_scale=1.0, post_norm="layer", post_g
                pre_norm="layer", pre_gamma=None, pre_beta=None, pre_eps=1e-5, want_y=True):
     """(y, h), of x's shape and type; y is None with want_y=False (a post-norm encoder only keeps h).  Differentiable."""
     xr, fr, index, cfg, w = _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_eps, pre_norm, pre_gamma, pre_beta, pre_eps)
-
-    def call():
-        y = _like(x) if want_y else None
-        h = _like(x)
-        sh.check(sh.lib().souffle_gated_norm_forward(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), h.data_ptr(), _stream(index)))
-        return y, h
     if torch.is_grad_enabled():
-        tensors = (x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta)
-        for v in tensors:
+        for v in (x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta):
             if v is not None and v.requires_grad:
                 numbers = dict(residual_scale=residual_scale, post_norm=post_norm, post_eps=post_eps, pre_norm=pre_norm, pre_eps=pre_eps)
-                return _Recorded.apply(call, numbers, *tensors)
-    return call()
+                return _Recorded.apply(want_y, numbers, x, f, gate, post_gamma, post_beta, pre_gamma, pre_beta)
+    y = _like(x) if want_y else None
+    h = _like(x)
+    sh.check(sh.lib().souffle_gated_norm_forward(cfg, w, xr.data_ptr(), fr.data_ptr(), sh.ptr(y), h.data_ptr(), _stream(index)))
+    return y, h
 
 
 @_on_device(0)

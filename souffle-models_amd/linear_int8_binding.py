@@ -105,23 +105,21 @@ def _overlap(a, rows_a, width_a, pitch_a, b, rows_b, width_b, pitch_b):
         return False
     if rows_a == 1:
         pitch_a = pitch_b
-    if rows_b == 1:
+    elif rows_b == 1:
         pitch_b = pitch_a
     gap = (b - a) % pitch_a
     return pitch_a != pitch_b or gap < width_a or gap + width_b > pitch_a
 
 
-def _check_apart(name, rows, ld, out, ldy, weight, bias, row_scale=None):
-    """out has no byte in common with an input (some are still read when it is written): the rows named `name`, row_scale, bias, weights."""
-    size, (M, N) = out.element_size(), out.shape
-    wide = rows.element_size()
-    if _overlap(rows.data_ptr(), rows.shape[0], rows.shape[1] * wide, ld * wide, out.data_ptr(), M, N * size, ldy * size):
-        raise ValueError("out must not overlap " + name)
-    for name, t in (("row_scale", row_scale), ("bias", bias), ("weight.packed", weight.packed), ("weight.scale", weight.scale)):
-        if t is not None:
-            nbytes = t.numel() * t.element_size()
-            if _overlap(t.data_ptr(), 1, nbytes, nbytes, out.data_ptr(), M, N * size, ldy * size):
-                raise ValueError("out must not overlap " + name)
+def _check_apart(at, M, width, pitch, named, *others):
+    """out (address, rows, bytes of a row, distance of the rows) has no byte in common with an input, as some are still read when
+    it is written: `named`, rows like out's with a name in front, and the others (name, address or None, bytes)."""
+    end = at + (M - 1) * pitch + width
+    if named[1] < end and at < named[1] + (M - 1) * named[3] + named[2] and _overlap(named[1], M, named[2], named[3], at, M, width, pitch):
+        raise ValueError("out must not overlap " + named[0])
+    for name, address, nbytes in others:
+        if address and address < end and at < address + nbytes and _overlap(address, 1, nbytes, nbytes, at, M, width, pitch):
+            raise ValueError("out must not overlap " + name)
 
 
 def pack_weight(weight_q, scale):
@@ -197,10 +195,12 @@ def gemm_int8(q, row_scale, weight, *, bias=None, act=None, dtype=torch.float16,
     b, a = _epilogue(bias, act, N, dtype, index)
     given = out is not None
     out, ldy = _output(out, q, M, N, dtype, index)
+    q_ptr, scale_ptr, out_ptr = q.data_ptr(), row_scale.data_ptr(), out.data_ptr()
     if given:
-        _check_apart("q", q, ldq, out, ldy, weight, bias, row_scale)
-    sh.check(sh.lib().souffle_gemm_int8(q.data_ptr(), ldq, row_scale.data_ptr(), packed, scale, b, a, out.data_ptr(), _DTYPES[dtype], ldy, M, N, K,
-                                        _stream(index)))
+        size = dtype.itemsize
+        _check_apart(out_ptr, M, N * size, ldy * size, ("q", q_ptr, K, ldq), ("row_scale", scale_ptr, 4 * M), ("bias", b, size * N),
+                     ("weight.packed", packed, weight.packed.numel()), ("weight.scale", scale, 4 * N))
+    sh.check(sh.lib().souffle_gemm_int8(q_ptr, ldq, scale_ptr, packed, scale, b, a, out_ptr, _DTYPES[dtype], ldy, M, N, K, _stream(index)))
     return out
 
 
@@ -221,10 +221,12 @@ def linear_int8(x, weight, *, bias=None, act=None, out=None):
     b, a = _epilogue(bias, act, N, x.dtype, index)
     given = out is not None
     out, ldy = _output(out, x, M, N, x.dtype, index)
+    x_ptr, out_ptr = x.data_ptr(), out.data_ptr()
     if given:
-        _check_apart("x", x, ld, out, ldy, weight, bias)
+        size = x.dtype.itemsize
+        _check_apart(out_ptr, M, N * size, ldy * size, ("x", x_ptr, K * size, ld * size), ("bias", b, size * N),
+                     ("weight.packed", packed, weight.packed.numel()), ("weight.scale", scale, 4 * N))
     nbytes = _workspace_bytes(M, N, K)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    sh.check(sh.lib().souffle_linear_int8(x.data_ptr(), ld, packed, scale, b, a, out.data_ptr(), _DTYPES[x.dtype], ldy, M, N, K, sh.ptr(ws), nbytes,
-                                          _stream(index)))
+    sh.check(sh.lib().souffle_linear_int8(x_ptr, ld, packed, scale, b, a, out_ptr, _DTYPES[x.dtype], ldy, M, N, K, sh.ptr(ws), nbytes, _stream(index)))
     return out
