@@ -397,6 +397,7 @@ enum { SOUFFLE_F16 = 0, SOUFFLE_BF16 = 1, SOUFFLE_F32 = 2 };
  * output channel; the sums are exact 32-bit integers.  K <= 131071, M <= 2^30.
  * A row x becomes q = round_half_even(x / s) with s = max(fp32(max |x| / 127), 2^-100): the rounding of the real quotient.
  * A row that holds a NaN or an infinity gets s = NaN (and q = 0), so that all results computed from it are NaN.
+ * The epilogue is in fp32, (sum * t[n]) * s[m] + bias[n]: sum * t[n] has to stay below 2^128, as it does for any weights below 2^103.
  * q lies in rows of ldq bytes, ldq a multiple of 16 and at least K rounded up to 64; the bytes behind K are multiplied
  * by zeros, whatever they hold.
  * No output overlaps an input.

@@ -131,8 +131,10 @@ __device__ __forceinline__ float normalize(float (&v)[NV][8], int kind, float ep
   return r;
 }
 
-// The next row is asked for while the present one is reduced.  16384 x 4096 bf16
-// takes 101 to 108 us, 537 MB at 5.0 to 5.3 TB/s (a large copy: 5.05); 4096 x 768 fp16 8.4 us, of which some 3 are the start and the end.
+// Where a slot has several rows, the next one is asked for while the present one is reduced.  16384 x 4096 bf16
+// takes 108 us (median; 105 at best), 537 MB at 5.0 TB/s (a large copy: 5.05).  4096 x 768 fp16 takes 8.4 to 9.0 us, of which some 3 are the start and
+// the end: one row per slot there, so nothing overlaps.  With fp32 rows of more than 8192 elements (two vectors a thread, 1024 threads, 128 registers) 114 to 160
+// registers a lane do not fit: 1024 x 16384 takes 166 us, three times its bytes.
 template <class T, int TPR, int NV, int WG, bool OUT8, RowForm FORM>
 __global__ void __launch_bounds__(WG) k_gated_norm(const FwdArgs a) {
   typedef typename Vec8<T>::type V;
@@ -257,8 +259,11 @@ struct BwdArgs {
 // Several rows at a time (one per slot of TPR threads), slots in step, so that a barrier of the workgroup serves them all.
 // Rows that share a gate row are taken in one go by all slots, or, where there are few of them (ROW_GATES), by one
 // slot each, which loads the gate with its row and writes the gate's gradient itself.
-// 8192 x 4096 bf16 takes 83 to 87 us, 403 MB at 4.6 to 4.9 TB/s.  With few rows per workgroup the arithmetic and the barriers of a
-// turn count instead, some 4 us for eight waves: 1182 x 1001 fp32, two turns, 16.6 us.
+// 8192 x 4096 bf16 takes 85 us (median, alone), 403 MB at 4.7 TB/s.  With few rows per workgroup the arithmetic and the barriers of a
+// turn count instead, some 4 us for eight waves: 1182 x 1001 fp32, two turns, 16.8 us.
+// Two vectors a thread hold five sums of 16 elements beside four rows and four vectors of parameters.  Registers a lane that do not fit: rows of
+// 4097 to 8192 elements 158 in fp32 (2048 x 8192: 128 us, bytes 80), 4 to 26 in 16 bits (55 us, bytes 40); beyond 8192 349 to 525
+// (1024 x 16384: 561 us in fp32, 335 in fp16, bytes 80 and 40); with ROW_GATES 0 to 7 and 295 to 386.
 template <class T, int TPR, int NV, int WG, RowForm FORM, bool KEEP, bool ROW_GATES>
 __global__ void __launch_bounds__(WG) k_gated_norm_grad(const BwdArgs a) {
   typedef typename Vec8<T>::type V;
@@ -557,7 +562,9 @@ static int check_vectors(const souffle_gated_norm_cfg *c, const souffle_gated_no
 template <RowForm FORM, class T, int TPR, int NV, int WG>
 static int launch_fwd(FwdArgs a, int num_cus, hipStream_t st) {
   constexpr int kSlots = WG / TPR;
-  const long long slots = (long long)num_cus * (2048 / WG) * kSlots;      // row slots that are resident at once
+  // Row slots, counted as if 2048 threads of a CU were resident.  The kernels' registers let 512 to 1536 stand (2 to 6 waves a SIMD), so just below
+  // this many rows the slots of one row each run in two to four rounds.
+  const long long slots = (long long)num_cus * (2048 / WG) * kSlots;
   a.rows_per_slot = (int)std::max<long long>(1, (a.rows + slots - 1) / slots);
   const int grid = (int)(((long long)a.rows + (long long)a.rows_per_slot * kSlots - 1) / ((long long)a.rows_per_slot * kSlots));
   if (a.q) hipLaunchKernelGGL((k_gated_norm<T, TPR, NV, WG, true, FORM>), dim3(grid), dim3(WG), 0, st, a);
@@ -567,8 +574,9 @@ static int launch_fwd(FwdArgs a, int num_cus, hipStream_t st) {
 }
 template <RowForm FORM, class T>
 static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
-  // One vector of 8 per thread in fp32, two in the 16-bit types from 513 elements on (measured: 4096 x 4096 fp32 48.6 us with one
-  // and 55.5 with two, which leave two waves per SIMD; 8192 x 4096 bf16 49.3 and 45.3, where two halve the waves of a sum).  Rows of up to
+  // One vector of 8 per thread in fp32, two in the 16-bit types from 513 elements on except 1025 to 2048 (measured: 4096 x 4096 fp32 48.6 us with one
+  // and 55.5 with two, which leave two waves per SIMD; 8192 x 4096 bf16 49.3 and 45.3, where two halve the waves of a sum; fp32 4096 x 768 12.0 with
+  // 128 threads and 13.5 with 64, 4096 x 2048 23.6 with 256 and 26.2 with 128; fp16 4096 x 2048 15.8 with 256 and 15.2 with 128).  Rows of up to
   // 256 elements share a wave, 16 threads each: 262144 x 64 fp16 32 us (106 with 64 threads), 131072 x 256 fp16 45 (60), fp32 117 (114).
   if constexpr (sizeof(T) == 4) {
     if (a.cols <= 128) return launch_fwd<FORM, T, 16, 1, 256>(a, num_cus, st);
@@ -596,8 +604,9 @@ static int forward(const FwdArgs &a, int num_cus, hipStream_t st) {
   return a.cols % 8 ? forward<kRagged, T>(a, num_cus, st) : forward<kWhole, T>(a, num_cus, st);
 }
 
-// How the rows are cut into chunks, one workgroup each: about `want` of them, none across gate rows unless it holds
-// whole gate rows.
+// How the rows are cut into chunks, one workgroup each: at most `want` of them, none across gate rows unless it holds
+// whole gate rows.  (With a gradient of the gate, 129 to 255 gate rows are that many chunks and 257 are 129: 130 | 256 | 257 gate rows of 200 x 768
+// fp16 take 137 | 146 | 269 us.)
 struct Chunks {
   int count, rows, per_gate;
 };

@@ -105,7 +105,7 @@ __device__ __forceinline__ size_t packed_at(int k, int n, int kblocks) {
 
 // Weights, once per model: a workgroup takes 64 columns, its waves parts of K; scale and rounding per column.  W = int8_t: packing alone.
 // 16 loads of a thread are under way at once (none behind a branch; what lies outside is read at the border and counts as 0).
-// 4096 x 4096 fp16: 67 us, of int8: 27 us.
+// 4096 x 4096 fp16: 65 us, of int8: 27 us; the bytes alone would take 10 (64 workgroups on 256 CUs that read every weight twice).
 constexpr int kPackParts = 16;
 template <class W>
 __global__ void __launch_bounds__(kPackParts * 64) k_pack_weight(const W *w, long long ldw, int8_t *packed, float *scale, int K, int N) {
@@ -164,10 +164,11 @@ struct Args {
 };
 
 // 0.5 v (1 + erf(v / sqrt 2)) as max(v, 0) - 0.5 z erfc(z / sqrt 2), z = |v|: no digits are lost in the negative tail.  erfc(z / sqrt 2) =
-// exp(-z^2 / 2) times a function that is smooth in t = 1 / (1 + 0.35 z) (the classical substitution), here half of it divided by t as
-// a polynomial of degree 8 fitted for z in 0..20 with the least largest relative error, 4.4e-8.  In all within 3 roundings of |v|, and 1e-6 of
-// the result for z <= 4.  17 instructions and two at quarter rate, no branch: 8192 x 4096 -> 4096 takes 127 us with
-// it, 137 with the library's erf, whose two ranges a wave both runs through.
+// exp(-z^2 / 2) times a function that is smooth in t = 1 / (1 + p z) (the substitution of Abramowitz and Stegun 7.1.25 to 7.1.28, with p = 0.35
+// here), half of it divided by t as a polynomial of degree 8 fitted for z in 0..20 for the least largest relative error: 5.2e-8 with
+// the constants as they are rounded to fp32.  In all within 3 roundings of |v|, and 1e-6 of the result for z <= 4.  17 instructions and two at
+// quarter rate, no branch: 8192 x 4096 -> 4096 takes 130 us with it and 114 without an activation (each call alone); the library's erf,
+// whose two ranges a wave both runs through, was 10 us slower than it in a build that differed in nothing else.
 __device__ __forceinline__ float gelu_exact(float v) {
   const float z = __builtin_fminf(__builtin_fabsf(v), 20.0f), t = __builtin_amdgcn_rcpf(__builtin_fmaf(z, 0.35f, 1.0f));
   constexpr float c[9] = {0.13962258398f, 0.13983604312f, 0.12006171793f, 0.10442747176f, -0.02011764981f, 0.15416617692f, -0.25073748827f, 0.14127224684f,
@@ -470,8 +471,8 @@ __device__ const int8_t zero_bytes[16] __attribute__((aligned(16))) = {};
 // direct loads, two steps ahead; the packed weights go straight into registers one step ahead, a wave's 64 columns being 4 KB in a
 // row per 64 of K: through LDS as well they would double its traffic, which at 128 bytes a cycle is
 // what runs out first (a 256 x 256 tile then asks for 64 + 32 + 32 bytes per cycle of matrix instructions).  8192 x 4096 x 4096 takes
-// 110 us (2500 TOP/s): the matrix cores are busy in 73 % of the cycles, LDS has no conflicts, 202 MB are read; without any load in
-// the loop it would be 87 us.
+// 114 us alone (median; 2410 TOP/s) and 122 to 129 in a row of calls, where the clock sinks (the library's product of these sizes 131 and 137):
+// the matrix cores are busy in 73 % of the cycles, LDS has no conflicts, 202 MB are read; without any load in the loop it would be 87 us.
 //
 // LDS stage [BM rows][8 slots of 16 bytes]: slot p of row r holds bytes 16 (p ^ (r / 2 % 8)) .. + 15 of the row's 128, so that the 16
 // rows of an operand read lie in different banks (64 banks are two rows); a direct load of 8 rows x 128 bytes fills 1 KB.
@@ -686,13 +687,15 @@ static int launch_tile(Args a, hipStream_t st) {
 }
 static long long tiles(int M, int rows, int N, int cols) { return (long long)((M + rows - 1) / rows) * ((N + cols - 1) / cols); }
 
-// Which kernel: the one with the most work per workgroup that still gives the CUs enough workgroups.  Measured alone on the GPU (bf16
-// out, us; split = 32 x 32 / 32 x 64 with the waves along K, tiles of 64 x 128 with four waves | with two | 128 x 128 | 256 x 256):
+// Which kernel: the one with the most work per workgroup that still gives the CUs enough workgroups.  Measured on the GPU (bf16
+// out, us, the best of several runs; split = 32 x 32 / 32 x 64 with the waves along K, tiles of 64 x 128 with four waves | with two | 128 x 128 | 256 x 256):
 //   64 x 4096 x 4096      7.5 /  8.3   15.3 | 17.4 | 21.0 | 44.7       512 x 4096 x 4096    39 / 25   16.3 | 18.3 | 21.8 | 48.2
 //   384 x 768 x 768       4.3 /  3.7    5.7 |  6.6 |  7.8 | 15.2       1024 x 768 x 2304    15 / 10    8.4 |  8.2 |  7.8 | 14.5
 //   8192 x 768 x 2304      99 /   62   30.1 | 26.5 | 26.7 | 30.2       5760 x 1600 x 1925   85 / 63   43.5 | 37.3 | 33.6 | 32.7
 //   8192 x 4096 x 4096    315 (per 64 x 64)  184 | 149 | 142 | 112      600 x 2048 x 8192   -  / 35   21.3 | 17.4 | 19.1 | 24.0
 //   4096 x 768 x 768       - / 12.6   8.5 |  8.4 |  7.5 | 13.4       5000 x 8192 x 800    - / 112  68.8 | 48.7 | 55.2 | 72.0
+// Between the smallest and the largest products these stay at two to four times the floor: output tiles are whole, so the last round of
+// workgroups is part empty, and with few steps of K nothing hides a workgroup's first loads and its epilogue.
 // (8192 x 768 x 2304: 288 tiles of 256 x 256 on 256 CUs: the second round is an eighth full; 600 x 2048 x 8192: 320 tiles of
 // 128 x 128, so some CUs get two where tiles of 64 rows give them three halves.)
 template <class T>
@@ -715,7 +718,8 @@ static int gemm(const Args &a, int dtype, hipStream_t st) {
 // Whether the product's workgroups quantise the rows themselves (one launch, no workspace).  Measured on the GPU in one launch and in
 // two, us: 1 x 768 -> 2304 3.7 and 5.0, 2 x 4096 -> 8192 9.1 and 10.1, 4 x 4096 -> 4096 9.0 and 8.9, 8 x 4096 -> 4096 11.5 and 9.2, 16 x 1024 ->
 // 4096 6.0 and 6.0; tiles of 32 rows: 32 x 512 -> 512 5.7 and 6.4, 384 x 768 -> 768 7.8 and 7.3, 128 x 1024 -> 4096 8.1 and 7.6, 333 x 1000 ->
-// 1111 fp32 8.4 and 7.7, 640 x 768 -> 768 7.7 and 7.7.  One call after another, which the host bounds, takes 8.8 and 12.9 in all of these.
+// 1111 fp32 8.4 and 7.7, 640 x 768 -> 768 7.7 and 7.7 (captured in a graph: 384 rows 7.7 and 7.1, 128 rows 8.1 and 7.3, 32 rows 6.1 and 6.5).
+// One call after another, which the host bounds, takes 8.8 and 12.9 in all of these.
 constexpr int kOneRound = 256;      // workgroups, one per CU: 98 KB of LDS each
 static bool rows_in_kernel(int M, int N, int K) {
   return M <= 16 ? (long long)M * K <= 16384 : K <= kRowsK && tiles(M, 32, N, 64) <= kOneRound;
