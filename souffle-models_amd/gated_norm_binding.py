@@ -5,7 +5,8 @@ between, forward and backward (a wrapper over the C ABI; the reference has no co
     y, q, s = gated_norm_int8(x, f, gate=g, ...)    # h as 8-bit rows for linear_int8_binding.gemm_int8
     grads = gated_norm_backward(dy, dh, x, f, gate=g, ...)
 
-x is the residual stream and f the block's output, [..., D] in fp16, bf16 or fp32; every vector has their type.  Keywords
+x is the residual stream and f the block's output, [..., D] in fp16, bf16 or fp32, rows at one distance (contiguous, or a slice such as
+x[..., a:b] or x[:, -1:]); every vector has their type.  Keywords
 of all three:
     post_norm, pre_norm     "layer", "rms"; post_norm also None
     post_gamma, post_beta, pre_gamma, pre_beta      [D] or None

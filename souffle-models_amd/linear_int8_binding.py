@@ -6,7 +6,7 @@
     y = gemm_int8(q, s, w, dtype=torch.float16)     #   (or comes from gated_norm_binding.gated_norm_int8)
 
 A row x is held as q = round_half_even(x / s), s = max(max|x| / 127, 2^-100) in fp32, a weight column likewise; products
-sum in exact 32-bit integers.  A row with a NaN or an infinity gives a row of NaN.  Work is queued on the current
+sum in exact 32-bit integers.  x [..., K] may be any slice whose rows lie at one distance (x[..., a:b], x[:, -1:]).  A row with a NaN or an infinity gives a row of NaN.  Work is queued on the current
 stream of the tensors' device; nothing is kept between calls, so calls may overlap on several streams and be captured.
 They are for inference: autograd does not record them, so their results require no gradient, whatever x requires.
 """
@@ -47,17 +47,22 @@ def _check_cuda(name, t, index=None):
 
 def _rows(name, t):
     """(t as [rows, columns] with adjacent columns, distance of its rows in elements)."""
-    if t.dim() == 2:
-        rows, cols = t.shape
-        if cols > 1 and t.stride(1) != 1:
-            raise ValueError("the columns of %s must be adjacent" % name)
-        ld = t.stride(0) if rows > 1 else cols
-        if ld < cols:
-            raise ValueError("the rows of %s overlap" % name)
-        return t, ld
-    if t.dim() < 1 or not t.is_contiguous():
-        raise ValueError("%s must be [rows, columns], or contiguous with another number of dimensions" % name)
-    return t.view(t.shape[:-1].numel(), t.shape[-1]), t.shape[-1]
+    if t.dim() != 2:
+        if t.dim() < 1:
+            raise ValueError("%s must have at least one dimension" % name)
+        if t.is_contiguous():
+            return t.view(t.shape[:-1].numel(), t.shape[-1]), t.shape[-1]
+        try:
+            t = t.view(t.shape[:-1].numel(), t.shape[-1])
+        except RuntimeError:
+            raise ValueError("the rows of %s must lie at one distance" % name) from None
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError("the columns of %s must be adjacent" % name)
+    ld = t.stride(0) if rows > 1 else cols
+    if ld < cols:
+        raise ValueError("the rows of %s overlap" % name)
+    return t, ld
 
 
 def _check_weight(w, index):
@@ -152,7 +157,7 @@ def quantize_weight(weight):
 
 
 def quantize_rows(x):
-    """(q, row_scale) of x [..., K] (more than two dimensions: contiguous): q [rows, K] int8 in rows that lie K rounded
+    """(q, row_scale) of x [..., K] (rows at one distance): q [rows, K] int8 in rows that lie K rounded
     up to 64 bytes apart, row_scale [rows] float32."""
     index = _check_cuda("x", x)
     if x.dtype not in _DTYPES:

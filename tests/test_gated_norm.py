@@ -497,6 +497,42 @@ def test_no_rows_and_leading_dimensions():
     assert y.shape == x.shape and torch.equal(y.view(6, 40), y2) and torch.equal(h.view(6, 40), h2)
 
 
+def test_rows_at_one_distance():
+    """Which tensors are rows at one distance, without a copy."""
+    import linear_int8_binding as lb
+    t = torch.arange(4 * 6 * 10).view(4, 6, 10)
+    for v, ld in ((t, 10), (t[..., 2:7], 10), (t[:, -1:], 60), (t[:, -1], 60), (t[:1, 1:3, :9], 10), (t[2, 3], 10), (t[2:3, 4:5, 3:5], 2), (t[:, :, :1], 10),
+                  (t.view(2, 2, 6, 10)[..., 1:4], 10), (t[:0, :, 1:3], None), (t[:, :, 3:3], None)):
+        rows, got = lb._rows("t", v)
+        assert rows.dim() == 2 and torch.equal(rows, v.reshape(v.shape[:-1].numel(), v.shape[-1])) and (not v.numel() or rows.data_ptr() == v.data_ptr())
+        assert ld is None or got == ld
+        if v.numel():
+            assert torch.equal(torch.as_strided(v, rows.shape, (got, 1), v.storage_offset()), rows)
+    for bad in (t[:, 1:3], t.transpose(0, 1), t.transpose(1, 2), t[:1].expand(4, 6, 10), t[..., ::2], t.flip(0)[0, 0, 0], t[0, 0, ::2]):
+        with pytest.raises(ValueError):
+            lb._rows("t", bad)
+
+
+@gpu
+def test_slices_of_three_dimensions():
+    announce("gated norm and 8-bit layer: slices of [B, S, D]")
+    import gated_norm_binding as gn
+    import linear_int8_binding as lb
+    wide = [values(50 + i, 4, 6, 90, dtype=torch.float16).cuda() for i in range(4)]
+    w = lb.quantize_weight(values(60, 77, 40).cuda())
+    gate = values(61, 4, 77, dtype=torch.float16).cuda()
+    for at in (lambda v: v[..., 5:82], lambda v: v[:, -1:, 5:82], lambda v: v[1:2, 2:4, :77].expand(1, 2, 77)):
+        x, f, dy, dh = (at(v) for v in wide)
+        near = [v.contiguous() for v in (x, f, dy, dh)]
+        p = dict(gate=gate if x.shape[0] == 4 else gate[0])
+        for a, b in ((gn.gated_norm(x, f, **p), gn.gated_norm(*near[:2], **p)), (gn.gated_norm_int8(x, f, **p), gn.gated_norm_int8(*near[:2], **p)),
+                     (gn.gated_norm_backward(dy, dh, x, f, **p).values(), gn.gated_norm_backward(near[2], near[3], *near[:2], **p).values()),
+                     (lb.quantize_rows(x), lb.quantize_rows(near[0])), ((lb.linear_int8(x, w),), (lb.linear_int8(near[0], w),))):
+            for u, v in zip(a, b):
+                assert (u is None and v is None) or (u.shape == v.shape and torch.equal(u, v))
+        assert gn.gated_norm(x, f)[0].shape == x.shape
+
+
 @gpu
 def test_rows_beyond_two_gib():
     announce("gated norm: offsets beyond 2^31")
