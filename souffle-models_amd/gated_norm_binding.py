@@ -84,7 +84,8 @@ def _like(x):
 def _setup(x, f, gate, residual_scale, post_norm, post_gamma, post_beta, post_eps, pre_norm, pre_gamma, pre_beta, pre_eps):
     """(x and f as rows, index of their device, cfg, vectors)."""
     index = _check_cuda("x", x)
-    _check_cuda("f", f, index)
+    if not isinstance(f, torch.Tensor) or f.get_device() != index:
+        _check_cuda("f", f, index)
     dtype = x.dtype
     if dtype not in _DTYPES or f.dtype != dtype:
         raise TypeError("x and f must both be float16, bfloat16 or float32")
